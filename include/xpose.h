@@ -354,6 +354,147 @@ int xp_kv_append_rows(float* cache, const float* src, uint32_t n_tokens, uint32_
 int xp_embed_lookup_rows(float* out, const float* table, const uint32_t* tokens, uint32_t n_tokens,
                          uint32_t n, uint32_t vocab, xp_stream stream);
 
+/* ---- packed rows and paged caches -------------------------------------------
+ * Operators of a server of many sequences, whose rows lie packed one sequence
+ * after the other and whose keys and values lie in pages. No reference
+ * counterpart: the reference decodes one sequence over a dense cache
+ * (decode.hpp:605-676); its single-sequence forms are xp_rope_prefill,
+ * xp_kv_append_f16 and xp_attention_decode.
+ *
+ * None of these calls allocates, synchronises or keeps anything: they may be
+ * captured into a graph, and calls on different streams do not meet unless
+ * their arguments do. What lies in device memory is not seen by the host's
+ * checks; the kernels bound it themselves (each entry says what becomes of a
+ * value out of range), so that no call reads or writes past the descriptors.
+ * A call whose n_tokens or n_seq is 0 does nothing.
+ *
+ * The memory has to be the current device's. A stream of another device, or an
+ * output that lies on another one, is refused with XP_E_ARG. */
+enum xp_elem { XP_ELEM_F32 = 0, XP_ELEM_F16 = 1, XP_ELEM_BF16 = 2, XP_ELEM_I8 = 3, XP_ELEM_E4M3 = 4 };
+
+/* Rows of heads: token t's head h at data + (t stride + h head_dim) elements.
+ * elem is F32, F16 or BF16; data 16-byte aligned and stride a multiple of 16
+ * bytes and at least heads * head_dim (a larger one steps over what a fused
+ * product leaves between). */
+typedef struct {
+    void*    data;
+    uint64_t stride;
+    uint32_t heads;
+    int32_t  elem;          /* xp_elem */
+} xp_rows;
+
+/* A cache: the row of kv head h in slot i of page p at
+ * ((p kv_heads + h) page_size + i) head_dim elements of k and of v. elem is
+ * F16 or BF16 (rows rounded to nearest even, scales NULL), or I8 or E4M3 with
+ * an f32 scale a row at (p kv_heads + h) page_size + i, value = code * scale:
+ *   I8    scale = f32(max|x| / 127), code = x / scale rounded to nearest even;
+ *   E4M3  scale = the least power of two with max|x| <= 448 scale, code =
+ *         x / scale rounded to nearest even.
+ * A row of zeros has scale 0. A row that holds an infinity or a NaN has scale
+ * NaN, so that all of it reads as NaN. page_size is a power of two from 16 to
+ * 1024, head_dim a multiple of 16 up to 256, every plane 16-byte aligned. */
+typedef struct {
+    void*    k;
+    void*    v;
+    float*   k_scale;
+    float*   v_scale;
+    int32_t  elem;          /* xp_elem */
+    uint32_t n_pages, page_size, kv_heads, head_dim;
+} xp_paged_kv;
+
+/* The sequences of one call. Sequence b's new tokens are the packed rows
+ * [cu[b], cu[b + 1]) of n_tokens; kv_len[b] is its length with them, so that
+ * row cu[b] + i is position kv_len[b] - (cu[b + 1] - cu[b]) + i. Position p is
+ * slot p % page_size of page pages[b * table + p / page_size]. All three arrays
+ * are in device memory. Rows at or behind cu[n_seq], and rows at a negative
+ * position, belong to no sequence: they are not read and not written. cu is
+ * taken as bounded to [0, n_tokens] and not to fall. A position whose page lies
+ * outside [0, n_pages) or past the table has no row. */
+typedef struct {
+    uint32_t       n_seq, n_tokens;
+    const int32_t* cu;      /* [n_seq + 1] */
+    const int32_t* kv_len;  /* [n_seq] */
+    const int32_t* pages;   /* [n_seq][table] */
+    uint32_t       table;
+} xp_paged_seqs;
+
+/* Rotary positions. Pair i of the rot_dim leading dims of a head (dims i and
+ * i + rot_dim / 2, or 2i and 2i + 1 when interleaved) is turned by pos f_i
+ * radians and multiplied by `magnitude` (0 = 1); the dims behind are copied.
+ * f_i = theta^(-2 i / rot_dim), times g + (1 - g) / factor with
+ *   PLAIN   g = 1;   LINEAR   g = 0;
+ *   BANDS   g = (r - low) / (high - low) bounded to [0, 1], r = original_len
+ *           f_i / 2 pi the pair's turns over the trained length;
+ *   PARTS   1 - g = (i - a) / (b - a) bounded to [0, 1], a and b the pair
+ *           indexes (floored, ceiled, bounded to [0, rot_dim - 1]; b - a at
+ *           least 0.001) of r = high and r = low. */
+enum xp_rope_layout { XP_ROPE_HALF = 0, XP_ROPE_INTERLEAVED = 1 };
+enum xp_rope_scaling { XP_ROPE_PLAIN = 0, XP_ROPE_LINEAR = 1, XP_ROPE_BANDS = 2, XP_ROPE_PARTS = 3 };
+typedef struct {
+    uint32_t rot_dim;       /* even, 2 .. head_dim */
+    int32_t  layout;        /* xp_rope_layout */
+    float    theta;         /* > 1 */
+    int32_t  scaling;       /* xp_rope_scaling */
+    float    factor;        /* >= 1 (not read when PLAIN) */
+    float    original_len;  /* > 0 (BANDS, PARTS) */
+    float    low, high;     /* 0 < low < high (BANDS, PARTS) */
+    float    magnitude;
+} xp_rope_spec;
+
+/* f_i of the rot_dim / 2 pairs, in radians a position (host only). */
+int xp_rope_frequencies(const xp_rope_spec* r, double* f, uint32_t n);
+/* Turns token t of q (and of k, in the same launch; k and k_out may both be
+ * NULL) by positions[t], a signed 32-bit position in device memory (a negative
+ * one turns back). Angles are exact to 2^-32 of a turn at any position. An
+ * output may be its input (turned in place) or not overlap it; it has its
+ * input's heads and elem. head_dim is even and at most 512; here data and
+ * stride need only the element's own alignment (fastest where both are
+ * multiples of 16 bytes). */
+int xp_rope_rows(const xp_rows* q_out, const xp_rows* q, const xp_rows* k_out, const xp_rows* k,
+                 const int32_t* positions, uint32_t n_tokens, uint32_t head_dim, const xp_rope_spec* r,
+                 xp_stream stream);
+/* Writes each new token's k and v row into the cache at its position,
+ * quantised as the cache has it. Rows whose position has no row in the cache
+ * are dropped. Where one call's tables give two tokens the same slot, what
+ * that slot holds afterwards is not defined. */
+int xp_paged_kv_write(const xp_paged_kv* c, const xp_paged_seqs* s, const xp_rows* k, const xp_rows* v,
+                      xp_stream stream);
+/* The inverse: each token's rows at its position in the cache, rounded once to
+ * the rows' elem; NaN where the position has no row. (With cu the sums of
+ * kv_len it reads whole sequences.) */
+int xp_paged_kv_read(const xp_paged_kv* c, const xp_paged_seqs* s, const xp_rows* k, const xp_rows* v,
+                     xp_stream stream);
+/* Attention of new tokens (one a sequence, a chunk, any mixture) over the
+ * cache, which holds their own rows too: the query at position p sees the
+ * positions (p - window, p] (all up to p when window is 0),
+ *   out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j,
+ * kv head h / (heads / kv_heads). A query that sees a position without a row
+ * in the cache gets NaN; what it does not see, not finite or not, does not
+ * reach it. Queries of any elem over F16, I8 and E4M3, of BF16 over BF16; F16
+ * queries are taken as they are, BF16 and F32 ones over a cache of another
+ * type as powers of two times F16 terms (F32: two terms). out has q's heads
+ * and elem and must not overlap q.
+ *
+ * workspace: where there are too few rows for the device's CUs the keys are
+ * split, and the parts meet in workspace_bytes (at least what
+ * xp_attention_workspace gives, 16-byte aligned). It is written before it is
+ * read in every call, and calls that may run at once need one each. NULL: the
+ * keys are not split. */
+int xp_attention_paged(const xp_rows* out, const xp_rows* q, const xp_paged_kv* c, const xp_paged_seqs* s,
+                       uint32_t window, float scale, void* workspace, size_t workspace_bytes,
+                       xp_stream stream);
+/* The same over packed prompts without a cache: sequence b's queries, keys and
+ * values are the rows [cu[b], cu[b + 1]), position 0 first. q, k, v and out are
+ * all F16 or all BF16; head_dim as for a cache. */
+int xp_attention_packed(const xp_rows* out, const xp_rows* q, const xp_rows* k, const xp_rows* v,
+                        uint32_t head_dim, uint32_t n_seq, uint32_t n_tokens, const int32_t* cu,
+                        uint32_t window, float scale, void* workspace, size_t workspace_bytes,
+                        xp_stream stream);
+/* Bytes that suffice for any call of these sizes, whatever its lengths (host
+ * only). */
+int xp_attention_workspace(uint32_t n_tokens, uint32_t n_seq, uint32_t heads, uint32_t kv_heads,
+                           uint32_t head_dim, size_t* bytes);
+
 /* ---- synthetic inputs (host side, counter-based, any thread count) ------ */
 /* Philox4x32-10 (Salmon et al., SC'11): out = philox(ctr, key). */
 void xp_philox4x32_10(const uint32_t ctr[4], const uint32_t key[2], uint32_t out[4]);

@@ -104,6 +104,35 @@ class RqTensor(C.Structure):
                 ("scale", C.c_void_p), ("bias", C.c_void_p)]
 
 
+# enum xp_elem / xp_rope_layout / xp_rope_scaling
+XP_ELEM_F32, XP_ELEM_F16, XP_ELEM_BF16, XP_ELEM_I8, XP_ELEM_E4M3 = range(5)
+XP_ROPE_HALF, XP_ROPE_INTERLEAVED = 0, 1
+XP_ROPE_PLAIN, XP_ROPE_LINEAR, XP_ROPE_BANDS, XP_ROPE_PARTS = range(4)
+
+
+class XpRows(C.Structure):
+    """xp_rows: packed rows of heads in device memory."""
+    _fields_ = [("data", C.c_void_p), ("stride", C.c_uint64), ("heads", C.c_uint32), ("elem", C.c_int32)]
+
+
+class XpPagedKv(C.Structure):
+    """xp_paged_kv: a cache of pages, with row scales when it has 8 bits."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("elem", C.c_int32)] + [(n, C.c_uint32) for n in ("n_pages", "page_size", "kv_heads", "head_dim")]
+
+
+class XpPagedSeqs(C.Structure):
+    """xp_paged_seqs: the sequences of one call, their arrays in device memory."""
+    _fields_ = [("n_seq", C.c_uint32), ("n_tokens", C.c_uint32), ("cu", C.c_void_p), ("kv_len", C.c_void_p),
+                ("pages", C.c_void_p), ("table", C.c_uint32)]
+
+
+class XpRope(C.Structure):
+    """xp_rope_spec: which dims are turned, and by which frequencies."""
+    _fields_ = [("rot_dim", C.c_uint32), ("layout", C.c_int32), ("theta", C.c_float), ("scaling", C.c_int32)] + \
+               [(n, C.c_float) for n in ("factor", "original_len", "low", "high", "magnitude")]
+
+
 class XpMetrics(C.Structure):
     _fields_ = [("ms", C.c_double), ("gpu_ms", C.c_double), ("sample_ms", C.c_double),
                 ("tokens_per_sec", C.c_double), ("position", C.c_uint32),
@@ -197,6 +226,14 @@ def _declare(lib: C.CDLL) -> None:
         "xp_gguf_meta_string": (i32, [vp, C.c_char_p, C.c_char_p, sz, P(sz)]),
         "xp_gguf_meta_array_length": (i32, [vp, C.c_char_p, P(C.c_uint64)]),
         "xp_dequantize": (i32, [u32, vp, vp, C.c_uint64]),
+        "xp_rope_frequencies": (i32, [P(XpRope), vp, u32]),
+        "xp_rope_rows": (i32, [P(XpRows), P(XpRows), P(XpRows), P(XpRows), vp, u32, u32, P(XpRope), vp]),
+        "xp_paged_kv_write": (i32, [P(XpPagedKv), P(XpPagedSeqs), P(XpRows), P(XpRows), vp]),
+        "xp_paged_kv_read": (i32, [P(XpPagedKv), P(XpPagedSeqs), P(XpRows), P(XpRows), vp]),
+        "xp_attention_paged": (i32, [P(XpRows), P(XpRows), P(XpPagedKv), P(XpPagedSeqs), u32, f32, vp, sz, vp]),
+        "xp_attention_packed": (i32, [P(XpRows), P(XpRows), P(XpRows), P(XpRows), u32, u32, u32, vp, u32, f32,
+                                      vp, sz, vp]),
+        "xp_attention_workspace": (i32, [u32, u32, u32, u32, u32, P(sz)]),
         "xp_softmax_rows_stats": (i32, [vp, vp, u32, u32, vp]),
         "xp_softmax_rows_apply": (i32, [vp, vp, u32, u32, vp]),
         "xp_attention_scores_prefill": (i32, [vp, vp, vp, u32, u32, u32, u32, u32, u32, u32, f32, vp]),
@@ -377,6 +414,22 @@ class DeviceBuffer:
 
 def synchronize() -> None:
     call("xp_synchronize")
+
+
+# ---- packed rows and paged caches -------------------------------------------
+
+def rope_frequencies(spec: XpRope) -> np.ndarray:
+    """Radians a position of each of the rot_dim / 2 pairs (xp_rope_frequencies)."""
+    out = np.empty(spec.rot_dim // 2, np.float64)
+    call("xp_rope_frequencies", spec, out.ctypes.data, out.size)
+    return out
+
+
+def attention_workspace(n_tokens: int, n_seq: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    """Bytes of workspace that suffice for xp_attention_paged / _packed calls of these sizes."""
+    n = C.c_size_t()
+    call("xp_attention_workspace", n_tokens, n_seq, heads, kv_heads, head_dim, C.byref(n))
+    return n.value
 
 
 # ---- synthetic inputs (host side; no GPU needed) ---------------------------
