@@ -467,8 +467,8 @@ int xp_paged_kv_read(const xp_paged_kv* c, const xp_paged_seqs* s, const xp_rows
 /* Attention of new tokens (one a sequence, a chunk, any mixture) over the
  * cache, which holds their own rows too: the query at position p sees the
  * positions (p - window, p] (all up to p when window is 0),
- *   out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j,
- * kv head h / (heads / kv_heads). A query that sees a position without a row
+ *   out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j,   scale > 0,
+ * kv head h / (heads / kv_heads). A sequence has at most 2^30 positions. A query that sees a position without a row
  * in the cache gets NaN; what it does not see, not finite or not, does not
  * reach it. Queries of any elem over F16, I8 and E4M3, of BF16 over BF16; F16
  * queries are taken as they are, BF16 and F32 ones over a cache of another

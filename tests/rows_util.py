@@ -124,10 +124,10 @@ class Seqs:
 
 def attend(q, keys, vals, scale, window, first):
     """One sequence in float64: q [new][heads][dim], keys and vals [position][kv_heads][dim], query i at
-    position first + i. Returns (out, sum_j p_j |v_j|, largest sum_d |q_d k_d| scale): the last two bound errors."""
+    position first + i. Returns (out, sum_j p_j |v_j|, (largest sum_d |q_d k_d| scale, floor)): the last two bound errors."""
     n, heads, dim = q.shape
     if keys.shape[0] == 0:
-        return torch.zeros_like(q), torch.zeros_like(q), torch.zeros(n, heads, 1, dtype=F64)
+        return torch.zeros_like(q), torch.zeros_like(q), torch.zeros(n, heads, 2, dtype=F64)
     group = heads // keys.shape[1]
     k, v = (x.repeat_interleave(group, 1).permute(1, 0, 2) for x in (keys, vals))
     place = first + torch.arange(n)[:, None]
@@ -143,13 +143,20 @@ def attend(q, keys, vals, scale, window, first):
         out[:, i] = (p[:, i, see][:, None] @ v[:, see])[:, 0]
         size[:, i] = (p[:, i, see][:, None] @ v[:, see].abs())[:, 0]
     most = (qs.abs() @ k.abs().transpose(1, 2) * scale).masked_fill(hidden, 0).nan_to_num(0).amax(-1)
-    return out.permute(1, 0, 2), size.permute(1, 0, 2), most.permute(1, 0)[..., None]
+    largest = torch.where(hidden[None, :, :], 0.0, v.abs().nan_to_num(0, posinf=0).amax(-1)[:, None, :]).amax(-1)
+    floor = 2.0 ** -30 * (~hidden).sum(-1)[None] * largest
+    return out.permute(1, 0, 2), size.permute(1, 0, 2), torch.stack((most, floor), -1).permute(1, 0, 2)
 
 
 def attention_bound(out, size, most, elem, op):
     """How far an attention output may be from attend()'s, per element, over at most 4096 keys of at most 256
-    dims. `size` = sum_j p_j |v_j|, `most` = S, the largest sum_d |q_d k_d| scale of a row. In units of `size`:
-      the weights' one rounding to the product's operands, half a step of `op` (two F16 terms: 2^-22);
+    dims. `size` = sum_j p_j |v_j|, `most` = S, the largest sum_d |q_d k_d| scale of a row, and the floor of its
+    weights: F16 ones, the largest at least 2^6 (after a shift that the quotient takes back, and over a power of two
+    at most twice the largest scale of an 8-bit cache), are off by 2^-24 at most however small they are: 2^-30 of the
+    largest value for each key (nothing beside the rest, unless the value of the key that has all the weight is 0).
+    In units of `size`:
+      the weights' one rounding to the product's operands, half a step of `op` (two F16 terms, the
+      first cut off and the second rounded: 2^-10 2^-11);
       the scores: sums of 256 exact products in blocks of 16 or more with at most 16 + 8 roundings of at most
       S 2^-24, the scales' two more: under 2^-19 S, which moves a weight and the sum of the weights by as
       much each; the exponential's argument, at most 2 S large, has 24 bits and its function 2 ulp: with the
@@ -157,5 +164,6 @@ def attention_bound(out, size, most, elem, op):
       the sums over the keys: one rounding for each block of 16 or more keys and one rescaling for each of 32
       or more, 4096 / 16 + 4096 / 32 + 16 < 2^9 of 2^-24: 2^-15.
     Last the output's own rounding, and half of the least F16 number."""
-    weights = 2.0 ** -22 if elem == "f32" else HALF[op]
-    return size * (weights + 2.0 ** -15 + 2.0 ** -17 * most) * 1.01 + HALF[elem] * out.abs() * 1.01 + 2.0 ** -25
+    weights = 2.0 ** -21 if elem == "f32" else HALF[op]
+    rel = weights + 2.0 ** -15 + 2.0 ** -17 * most[..., :1]
+    return (size * rel + (most[..., 1:] if op == "f16" else 0.0) + HALF[elem] * out.abs()) * 1.01 + 2.0 ** -25

@@ -24,10 +24,11 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
 # -packed-fp32-ops: never emit v_pk_{add,mul,fma}_f32 (the host pass warns
-# that it does not know the feature; that is harmless).
+# that it does not know the feature; that is harmless). -Wno-inline-asm: the
+# loads into LDS name m0, which they write, as clobbered; it is reserved.
 HIP_FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17", "-Wall",
-    "-Wno-unused-function", "-Xclang", "-target-feature", "-Xclang",
+    "-Wno-unused-function", "-Wno-inline-asm", "-Xclang", "-target-feature", "-Xclang",
     "-packed-fp32-ops", "-munsafe-fp-atomics",
 ]
 
@@ -35,7 +36,7 @@ LIB_SOURCES = ["runtime.cpp", "synth.cpp", "matvec.hip", "transformer.hip", "sam
                "sampling_chain.hip", "token_kernel.hip", "probe.hip", "batch_kernels.hip", "batch_step.hip",
                "batch.cpp", "prefill_engine.hip", "prefill.cpp", "gguf.cpp", "pack.cpp", "tokenizer.cpp", "repack.cpp", "native_quant.hip", "prefill_kernels.hip",
                "session_kernels.hip", "session.cpp",
-               "rows.cpp", "rope_rows.hip", "paged_kv.hip", "rows_attention.hip"]
+               "rows.cpp", "rope_rows.hip", "paged_kv.hip", "rows_attention.hip", "rows_attn_few.hip", "rows_attn_tile.hip"]
 
 
 def _run(cmd: list[str], verbose: bool) -> None:

@@ -5,83 +5,113 @@
 // sum make it one pass over the keys: when the maximum rises from m to m', what
 // has been summed is multiplied by exp(m - m').
 //
-// The simple form: a wave takes one query head of one token and its keys one
-// by one.
+// The products are made by two kernels, for few rows a sequence
+// (rows_attn_few.hip) and for many (rows_attn_tile.hip). Where the rows alone
+// leave CUs without work the keys are split, and a second kernel joins the parts.
 #include <algorithm>
 
-#include "xp_elem.hpp"
+#include "xp_rows_attn.hpp"
 
 namespace xp {
 namespace {
 
-struct AttnRows {
-    const void *q, *k, *v;         // k, v: the cache's planes, or the packed rows
-    void*       out;
-    const float *k_scale, *v_scale;
-    uint64_t    q_stride, k_stride, v_stride, out_stride;
-    const int32_t *cu, *kv_len;    // kv_len NULL: packed
-    PageMap     map;
-    uint32_t    n_seq, n_tokens, heads, kv_heads, head_dim, window;
-    float       scale;
-};
-constexpr int kMostDims = 256 / kWave;
+constexpr uint32_t kJoinThreads = 256, kJoinWaves = kJoinThreads / kWave;
 
-template <int Q, int KV, bool PAGED>
-__global__ __launch_bounds__(kWave) void rows_attention_kernel(AttnRows a) {
-    const uint32_t t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, D = a.head_dim;
-    const uint32_t kvh = h / (a.heads / a.kv_heads);
-    const uint32_t b = seq_of_row(a.cu, a.n_seq, a.n_tokens, t);
-    if (b >= a.n_seq) return;
-    const RowSpan r = row_span(a.cu, a.n_tokens, b);
-    const uint32_t n = r.end - r.first;
-    const int64_t p = row_position(PAGED ? a.kv_len[b] : int32_t(n), n, t - r.first);
-    if (p < 0) return;
-    float q[kMostDims], o[kMostDims];
-    const uint64_t qi = uint64_t(t) * a.q_stride + uint64_t(h) * D;
+// A workgroup joins the parts of one row: the sums relative to the largest
+// reference, each wave every fourth part.
+template <int DP>
+__global__ __launch_bounds__(kJoinThreads) void rows_attn_join_kernel(AttnRows a) {
+    constexpr int PER = DP / kWave;
+    __shared__ float s_o[kJoinWaves][DP];
+    __shared__ float s_l[kJoinWaves];
+    const uint32_t t = blockIdx.x / a.heads, head = blockIdx.x % a.heads, lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
+    const uint32_t seq = seq_of_row(a.cu, a.n_seq, a.n_tokens, t);
+    if (seq >= a.n_seq) return;
+    const TileSeq ts = tile_seq(a, seq);
+    if (ts.past + int32_t(t - ts.first) < 0) return;
+    const uint32_t group = a.heads / a.kv_heads, row = (t - ts.first) * group + head % group;
+    const uint32_t tile = row >> a.row_shift, r = row & ((1u << a.row_shift) - 1u), tile_rows = 1u << a.row_shift;
+    uint32_t n;
+    const uint32_t first = deal_first(a, seq, tile, head / group, &n);
+    if (n == 0 || uint64_t(first) + uint64_t(n - 1u) * a.kv_heads >= a.items) return;    // a cu that gives rows twice
+    const float* base = a.part + uint64_t(first) * part_floats(tile_rows, DP);
+    const uint64_t step = uint64_t(a.kv_heads) * part_floats(tile_rows, DP);
+    auto ml = [&](uint32_t p) { return reinterpret_cast<const float2*>(base + p * step + tile_rows * DP)[r]; };
+    float top = -INFINITY;
+    for (uint32_t p = lane; p < n; p += kWave) top = fmaxf(top, ml(p).x);
+    top = wave_max(top);
+    float o[PER] = {}, l = 0.0f;
+    for (uint32_t p = wave; p < n; p += kJoinWaves) {
+        const float2 w = ml(p);
+        if (w.x == -INFINITY) continue;            // it saw nothing
+        const float f = exp2_hw(w.x - top);
+        const float* x = base + p * step + r * DP + lane * PER;
+        l += w.y * f;
 #pragma unroll
-    for (int j = 0; j < kMostDims; ++j) {
-        const uint32_t d = lane + j * kWave;
-        q[j] = d < D ? load1<Q>(a.q, qi + d) : 0.0f;
-        o[j] = 0.0f;
+        for (int j = 0; j < PER; ++j) o[j] += x[j] * f;
     }
-    float m = -INFINITY, l = 0.0f;
-    bool whole = true;
-    for (int64_t j = a.window && p >= a.window ? p - a.window + 1 : 0; j <= p; ++j) {
-        uint64_t ki, vi;
-        float ks = 1.0f, vs = 1.0f;
-        if constexpr (PAGED) {
-            const int32_t g = page_of(a.map, b, j);
-            if (g < 0) {
-                whole = false;
-                break;
-            }
-            const uint64_t row = cache_row(uint32_t(g), a.kv_heads, kvh, a.map.page_shift, uint32_t(j) & ((1u << a.map.page_shift) - 1u));
-            ki = vi = row * D;
-            if constexpr (KV == XP_ELEM_I8 || KV == XP_ELEM_E4M3) ks = a.k_scale[row], vs = a.v_scale[row];
-        } else {
-            ki = uint64_t(r.first + j) * a.k_stride + uint64_t(kvh) * D;
-            vi = uint64_t(r.first + j) * a.v_stride + uint64_t(kvh) * D;
-        }
-        float s = 0.0f, v[kMostDims];
 #pragma unroll
-        for (int x = 0; x < kMostDims; ++x) {
-            const uint32_t d = lane + x * kWave;
-            if (d < D) s = fmaf(q[x], load1<KV>(a.k, ki + d), s);
-            v[x] = d < D ? load1<KV>(a.v, vi + d) : 0.0f;
-        }
-        s = wave_sum(s) * ks * a.scale;
-        const float top = fmaxf(m, s);
-        const float keep = top == m ? 1.0f : exp_hw(m - top), w = exp_hw(s - (top == -INFINITY ? 0.0f : top));
-        m = top;
-        l = l * keep + w;
+    for (int j = 0; j < PER; ++j) s_o[wave][lane * PER + j] = o[j];
+    if (lane == 0) s_l[wave] = l;
+    __syncthreads();
+    const uint32_t d = threadIdx.x * 4;
+    if (d >= a.head_dim) return;
+    f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
+    float sum = 0.0f;
 #pragma unroll
-        for (int x = 0; x < kMostDims; ++x) o[x] = o[x] * keep + w * (v[x] * vs);
+    for (uint32_t w = 0; w < kJoinWaves; ++w) {
+        sum += s_l[w];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += s_o[w][d + j];
     }
-    const float norm = whole ? (l > 0.0f || l != l ? 1.0f / l : 0.0f) : __uint_as_float(0x7FC00000u);
-    const uint64_t oi = uint64_t(t) * a.out_stride + uint64_t(h) * D;
-#pragma unroll
-    for (int x = 0; x < kMostDims; ++x)
-        if (lane + x * kWave < D) store1<Q>(a.out, oi + lane + x * kWave, o[x] * norm);
+    store_row4(a, t, head, d, v, sum);
+}
+
+// ---- which kernel, and whether to split ------------------------------------------
+struct AttnPlan {
+    bool     few;
+    uint32_t row_shift, items, target;     // items: the grid; target 0: the keys are not split
+    size_t   part_bytes;
+};
+constexpr uint32_t kCus = 256;
+// The tiles of a call, at most: every sequence with rows may leave one part-filled.
+uint64_t most_tiles(uint32_t n_tokens, uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t rows) {
+    return (uint64_t(n_tokens) * (heads / kv_heads) / rows + std::min(n_seq, n_tokens)) * kv_heads;
+}
+AttnPlan attn_plan(bool paged, uint32_t n_tokens, uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+    AttnPlan p{};
+    const uint64_t rows = uint64_t(n_tokens) * (heads / kv_heads);
+    p.few = paged && rows <= uint64_t(std::min(n_seq, n_tokens)) * 2 * kFewRows;
+    const uint32_t tile = p.few ? kFewRows : kTileRows;
+    p.row_shift = uint32_t(__builtin_ctz(tile));
+    const uint64_t tiles = most_tiles(n_tokens, n_seq, heads, kv_heads, tile);
+    const uint64_t enough = p.few ? 8 * kCus : 2 * kCus;
+    if (tiles < enough) {
+        p.target = p.few ? 4 * kCus : 2 * kCus;
+        p.part_bytes = size_t((tiles + p.target) * part_floats(tile, padded_dim(head_dim)) * sizeof(float));
+    }
+    p.items = uint32_t(std::min<uint64_t>(tiles + p.target, 0x7FFFFFFFu));
+    return p;
+}
+
+int attention_call(const char* fn, AttnRows a, const AttnPlan& plan, int cache, bool paged, void* workspace, hipStream_t st) {
+    AttnPlan p = plan;
+    if (!workspace) p.target = 0;
+    a.target = p.target;
+    a.part = static_cast<float*>(workspace);
+    a.row_shift = p.row_shift;
+    a.items = p.items;
+    const uint32_t dp = padded_dim(a.head_dim);
+    const uint32_t block = p.few ? kFewWaves * few_keys(dp, elem_bytes(cache)) : tile_keys_of(dp);
+    a.block_shift = uint32_t(__builtin_ctz(block));
+    XP_CHECK(p.few ? launch_few(a, cache, p.items, st) : launch_tile(a, cache, paged, p.items, st));
+    if (p.target == 0) return XP_OK;
+    const dim3 grid(a.n_tokens * a.heads);
+    if (dp == 64) hipLaunchKernelGGL((rows_attn_join_kernel<64>), grid, dim3(kJoinThreads), 0, st, a);
+    else if (dp == 128) hipLaunchKernelGGL((rows_attn_join_kernel<128>), grid, dim3(kJoinThreads), 0, st, a);
+    else hipLaunchKernelGGL((rows_attn_join_kernel<256>), grid, dim3(kJoinThreads), 0, st, a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return set_error(XP_E_HIP, "%s: kernel launch -> %s", fn, hipGetErrorString(e));
+    return XP_OK;
 }
 
 int check_attention(const char* fn, const xp_rows* out, const xp_rows* q, uint32_t head_dim, uint32_t kv_heads,
@@ -93,7 +123,7 @@ int check_attention(const char* fn, const xp_rows* out, const xp_rows* q, uint32
     if (q->heads % kv_heads) return set_error(XP_E_ARG, "%s: %u heads are no multiple of %u kv heads", fn, q->heads, kv_heads);
     if (uint64_t(n_tokens) * q->heads > 0x7FFFFFFFull)
         return set_error(XP_E_ARG, "%s: %u tokens of %u heads are over 2^31 - 1", fn, n_tokens, q->heads);
-    if (!(scale == scale) || scale - scale != 0.0f) return set_error(XP_E_ARG, "%s: scale is not finite", fn);
+    if (!(scale > 0.0f) || scale - scale != 0.0f) return set_error(XP_E_ARG, "%s: scale %g is not positive and finite", fn, double(scale));
     if (workspace) {
         size_t need = 0;
         XP_CHECK(xp_attention_workspace(n_tokens, n_seq, q->heads, kv_heads, head_dim, &need));
@@ -115,7 +145,8 @@ int xp_attention_workspace(uint32_t n_tokens, uint32_t n_seq, uint32_t heads, ui
     XP_REQUIRE(bytes, "bytes is null");
     XP_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%u heads are no multiple of %u kv heads", heads, kv_heads);
     XP_REQUIRE(head_dim > 0 && head_dim % 16 == 0 && head_dim <= 256, "head_dim %u is not a multiple of 16 up to 256", head_dim);
-    *bytes = 16;
+    *bytes = std::max<size_t>({16, attn_plan(true, n_tokens, n_seq, heads, kv_heads, head_dim).part_bytes,
+                               attn_plan(false, n_tokens, n_seq, heads, kv_heads, head_dim).part_bytes});
     return XP_OK;
 }
 
@@ -127,27 +158,13 @@ int xp_attention_paged(const xp_rows* out, const xp_rows* q, const xp_paged_kv* 
     XP_REQUIRE(c->elem != XP_ELEM_BF16 || q->elem == XP_ELEM_BF16, "a BF16 cache takes BF16 queries");
     if (s->n_tokens == 0 || s->n_seq == 0) return XP_OK;
     XP_CHECK(check_here(__func__, stream, out->data));
-    const AttnRows a{q->data, c->k, c->v, out->data, c->k_scale, c->v_scale, q->stride, 0, 0, out->stride, s->cu, s->kv_len,
-                     page_map(c, s), s->n_seq, s->n_tokens, q->heads, c->kv_heads, c->head_dim, window, scale};
-    const dim3 grid(s->n_tokens, q->heads);
-#define XP_PAGED(Q, KV) hipLaunchKernelGGL((rows_attention_kernel<Q, KV, true>), grid, dim3(kWave), 0, as_stream(stream), a)
-#define XP_PAGED_Q(KV)                                              \
-    if (q->elem == XP_ELEM_F32) XP_PAGED(XP_ELEM_F32, KV);          \
-    else if (q->elem == XP_ELEM_F16) XP_PAGED(XP_ELEM_F16, KV);     \
-    else XP_PAGED(XP_ELEM_BF16, KV);
-    if (c->elem == XP_ELEM_BF16) {
-        XP_PAGED(XP_ELEM_BF16, XP_ELEM_BF16);
-    } else if (c->elem == XP_ELEM_F16) {
-        XP_PAGED_Q(XP_ELEM_F16)
-    } else if (c->elem == XP_ELEM_I8) {
-        XP_PAGED_Q(XP_ELEM_I8)
-    } else {
-        XP_PAGED_Q(XP_ELEM_E4M3)
-    }
-#undef XP_PAGED_Q
-#undef XP_PAGED
-    XP_LAUNCHED();
-    return XP_OK;
+    AttnRows a{};
+    a.q = q->data, a.k = c->k, a.v = c->v, a.out = out->data, a.k_scale = c->k_scale, a.v_scale = c->v_scale;
+    a.q_stride = q->stride, a.out_stride = out->stride;
+    a.cu = s->cu, a.kv_len = s->kv_len, a.map = page_map(c, s), a.n_seq = s->n_seq, a.n_tokens = s->n_tokens;
+    a.heads = q->heads, a.kv_heads = c->kv_heads, a.head_dim = c->head_dim, a.window = window, a.q_elem = q->elem, a.scale = scale;
+    return attention_call(__func__, a, attn_plan(true, a.n_tokens, a.n_seq, a.heads, a.kv_heads, a.head_dim), c->elem, true, workspace,
+                          as_stream(stream));
 }
 
 int xp_attention_packed(const xp_rows* out, const xp_rows* q, const xp_rows* k, const xp_rows* v, uint32_t head_dim,
@@ -163,15 +180,13 @@ int xp_attention_packed(const xp_rows* out, const xp_rows* q, const xp_rows* k, 
     if (n_tokens == 0 || n_seq == 0) return XP_OK;
     XP_REQUIRE(cu, "cu is null");
     XP_CHECK(check_here(__func__, stream, out->data));
-    const AttnRows a{q->data, k->data, v->data, out->data, nullptr, nullptr, q->stride, k->stride, v->stride, out->stride, cu,
-                     nullptr, PageMap{}, n_seq, n_tokens, q->heads, k->heads, head_dim, window, scale};
-    const dim3 grid(n_tokens, q->heads);
-    if (q->elem == XP_ELEM_F16)
-        hipLaunchKernelGGL((rows_attention_kernel<XP_ELEM_F16, XP_ELEM_F16, false>), grid, dim3(kWave), 0, as_stream(stream), a);
-    else
-        hipLaunchKernelGGL((rows_attention_kernel<XP_ELEM_BF16, XP_ELEM_BF16, false>), grid, dim3(kWave), 0, as_stream(stream), a);
-    XP_LAUNCHED();
-    return XP_OK;
+    AttnRows a{};
+    a.q = q->data, a.k = k->data, a.v = v->data, a.out = out->data;
+    a.q_stride = q->stride, a.k_stride = k->stride, a.v_stride = v->stride, a.out_stride = out->stride;
+    a.cu = cu, a.n_seq = n_seq, a.n_tokens = n_tokens;
+    a.heads = q->heads, a.kv_heads = k->heads, a.head_dim = head_dim, a.window = window, a.q_elem = q->elem, a.scale = scale;
+    return attention_call(__func__, a, attn_plan(false, n_tokens, n_seq, a.heads, a.kv_heads, head_dim), k->elem, false, workspace,
+                          as_stream(stream));
 }
 
 }  // extern "C"
