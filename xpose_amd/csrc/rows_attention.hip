@@ -16,100 +16,124 @@ namespace xp {
 namespace {
 
 constexpr uint32_t kJoinThreads = 256, kJoinWaves = kJoinThreads / kWave;
+constexpr uint32_t kJoinSlices = 4;        // workgroups a tile
+constexpr int kJoinBatch = 16;             // parts that a wave reads at once
 
-// A workgroup joins the parts of one row: the sums relative to the largest
-// reference, each wave every fourth part.
+// Workgroup (slice, w) joins the tile that begins in run w and ends behind it, if
+// there is one: every kJoinSlices-th row: a wave a row, or, of few rows of many parts,
+// all four waves, every fourth part each.
 template <int DP>
 __global__ __launch_bounds__(kJoinThreads) void rows_attn_join_kernel(AttnRows a) {
     constexpr int PER = DP / kWave;
+    typedef float vec __attribute__((ext_vector_type(PER)));
     __shared__ float s_o[kJoinWaves][DP];
-    __shared__ float s_l[kJoinWaves];
-    const uint32_t t = blockIdx.x / a.heads, head = blockIdx.x % a.heads, lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
-    const uint32_t seq = seq_of_row(a.cu, a.n_seq, a.n_tokens, t);
-    if (seq >= a.n_seq) return;
-    const TileSeq ts = tile_seq(a, seq);
-    if (ts.past + int32_t(t - ts.first) < 0) return;
-    const uint32_t group = a.heads / a.kv_heads, row = (t - ts.first) * group + head % group;
-    const uint32_t tile = row >> a.row_shift, r = row & ((1u << a.row_shift) - 1u), tile_rows = 1u << a.row_shift;
-    uint32_t n;
-    const uint32_t first = deal_first(a, seq, tile, head / group, &n);
-    if (n == 0 || uint64_t(first) + uint64_t(n - 1u) * a.kv_heads >= a.items) return;    // a cu that gives rows twice
-    const float* base = a.part + uint64_t(first) * part_floats(tile_rows, DP);
-    const uint64_t step = uint64_t(a.kv_heads) * part_floats(tile_rows, DP);
-    auto ml = [&](uint32_t p) { return reinterpret_cast<const float2*>(base + p * step + tile_rows * DP)[r]; };
-    float top = -INFINITY;
-    for (uint32_t p = lane; p < n; p += kWave) top = fmaxf(top, ml(p).x);
-    top = wave_max(top);
-    float o[PER] = {}, l = 0.0f;
-    for (uint32_t p = wave; p < n; p += kJoinWaves) {
-        const float2 w = ml(p);
-        if (w.x == -INFINITY) continue;            // it saw nothing
-        const float f = exp2_hw(w.x - top);
-        const float* x = base + p * step + r * DP + lane * PER;
-        l += w.y * f;
+    __shared__ float2 s_ml[kJoinWaves];
+    const uint32_t lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), w0 = blockIdx.y;
+    const JoinTile p = reinterpret_cast<const JoinTile*>(a.part)[w0];
+    const uint32_t n = uniform(p.parts), r0 = p.r0, rows = uniform(p.rows), group = a.heads / a.kv_heads;
+    if (n < 2) return;
+    const uint64_t size = part_floats(1u << a.row_shift, DP);
+    const float* base = part_record(a, w0, false, size);
+    const bool all = n >= 2 * kJoinWaves && rows <= kJoinWaves * kJoinSlices;     // all waves a row
+    const uint32_t step = all ? kJoinWaves : 1u, at = all ? wave : 0u;
+    for (uint32_t r = blockIdx.x + (all ? 0u : wave * kJoinSlices); r < rows; r += kJoinSlices * (all ? 1u : kJoinWaves)) {
+        const uint32_t t = by_group(a, r0 + r), head = p.kv_head * group + (r0 + r - t * group);
+        float top = -INFINITY, l = 0.0f;
+        vec o{};
+        for (uint32_t i0 = at; i0 < n; i0 += step * kJoinBatch) {
+            float2 ml[kJoinBatch];
+            vec x[kJoinBatch];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) o[j] += x[j] * f;
+            for (int j = 0; j < kJoinBatch; ++j) {
+                const uint32_t i = min(i0 + j * step, n - 1u);
+                const float* rec = base + (2ull * i + (i == 0 ? 1u : 0u)) * size;
+                ml[j] = reinterpret_cast<const float2*>(rec + (size_t(DP) << a.row_shift))[r];
+                x[j] = *reinterpret_cast<const vec*>(rec + size_t(r) * DP + lane * PER);
+            }
+            float most = top;
+#pragma unroll
+            for (int j = 0; j < kJoinBatch; ++j) {
+                if (i0 + j * step >= n) ml[j] = {-INFINITY, 0.0f};
+                most = fmaxf(most, ml[j].x);
+            }
+            const float keep = top == -INFINITY ? 0.0f : exp2_hw(top - most);
+            l *= keep;
+            o *= keep;
+            top = most;
+#pragma unroll
+            for (int j = 0; j < kJoinBatch; ++j) {
+                const bool in = ml[j].x != -INFINITY;                // it saw something
+                const float f = in ? exp2_hw(ml[j].x - top) : 0.0f;
+                l += in ? ml[j].y * f : 0.0f;
+#pragma unroll
+                for (int e = 0; e < PER; ++e) o[e] += in ? x[j][e] * f : 0.0f;
+            }
+        }
+        if (all) __syncthreads();
+        *reinterpret_cast<vec*>(&s_o[wave][lane * PER]) = o;
+        if (lane == 0) s_ml[wave] = {top, l};
+        if (all) __syncthreads();
+        const uint32_t d = (all ? threadIdx.x : lane) * 4;
+        if (d < a.head_dim && p.past + int32_t(t) >= 0) {
+            const uint32_t v0 = all ? 0u : wave, v1 = all ? kJoinWaves : wave + 1u;
+            float most = -INFINITY, sum = 0.0f;
+            for (uint32_t v = v0; v < v1; ++v) most = fmaxf(most, s_ml[v].x);
+            f32x4 y{0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t v = v0; v < v1; ++v) {
+                const float2 ml = s_ml[v];
+                if (ml.x == -INFINITY) continue;
+                const float f = exp2_hw(ml.x - most);
+                sum += ml.y * f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] += s_o[v][d + j] * f;
+            }
+            store_row4(a, p.first + t, head, d, y, sum);
+        }
     }
-#pragma unroll
-    for (int j = 0; j < PER; ++j) s_o[wave][lane * PER + j] = o[j];
-    if (lane == 0) s_l[wave] = l;
-    __syncthreads();
-    const uint32_t d = threadIdx.x * 4;
-    if (d >= a.head_dim) return;
-    f32x4 v{0.0f, 0.0f, 0.0f, 0.0f};
-    float sum = 0.0f;
-#pragma unroll
-    for (uint32_t w = 0; w < kJoinWaves; ++w) {
-        sum += s_l[w];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += s_o[w][d + j];
-    }
-    store_row4(a, t, head, d, v, sum);
 }
 
-// ---- which kernel, and whether to split ------------------------------------------
+// ---- which kernel, and how the work is dealt ----------------------------------------
 struct AttnPlan {
     bool     few;
-    uint32_t row_shift, items, target;     // items: the grid; target 0: the keys are not split
+    uint32_t row_shift, tiles, target;     // the most tiles; target 0: a workgroup for each
     size_t   part_bytes;
 };
 constexpr uint32_t kCus = 256;
-// The tiles of a call, at most: every sequence with rows may leave one part-filled.
-uint64_t most_tiles(uint32_t n_tokens, uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t rows) {
-    return (uint64_t(n_tokens) * (heads / kv_heads) / rows + std::min(n_seq, n_tokens)) * kv_heads;
-}
 AttnPlan attn_plan(bool paged, uint32_t n_tokens, uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
     AttnPlan p{};
     const uint64_t rows = uint64_t(n_tokens) * (heads / kv_heads);
-    p.few = paged && rows <= uint64_t(std::min(n_seq, n_tokens)) * 2 * kFewRows;
+    const uint32_t seqs = std::min(n_seq, n_tokens);
+    p.few = paged && rows <= uint64_t(seqs) * 2 * kFewRows;
     const uint32_t tile = p.few ? kFewRows : kTileRows;
     p.row_shift = uint32_t(__builtin_ctz(tile));
-    const uint64_t tiles = most_tiles(n_tokens, n_seq, heads, kv_heads, tile);
-    const uint64_t enough = p.few ? 8 * kCus : 2 * kCus;
-    if (tiles < enough) {
-        p.target = p.few ? 4 * kCus : 2 * kCus;
-        p.part_bytes = size_t((tiles + p.target) * part_floats(tile, padded_dim(head_dim)) * sizeof(float));
+    // every sequence with rows may leave one tile part filled
+    const uint64_t tiles = (rows / tile + seqs) * kv_heads;
+    p.tiles = uint32_t(std::min<uint64_t>(tiles, 0x7FFFFFFFu));
+    if (tiles < (p.few ? 16 : 4) * kCus) {
+        p.target = padded_dim(head_dim) == 256 ? kCus : 2 * kCus;          // what fits the device at once
+        p.part_bytes = size_t(p.target) * (sizeof(JoinTile) + 2 * part_floats(tile, padded_dim(head_dim)) * sizeof(float));
     }
-    p.items = uint32_t(std::min<uint64_t>(tiles + p.target, 0x7FFFFFFFu));
     return p;
 }
 
-int attention_call(const char* fn, AttnRows a, const AttnPlan& plan, int cache, bool paged, void* workspace, hipStream_t st) {
-    AttnPlan p = plan;
-    if (!workspace) p.target = 0;
-    a.target = p.target;
-    a.part = static_cast<float*>(workspace);
-    a.row_shift = p.row_shift;
-    a.items = p.items;
+int attention_call(const char* fn, AttnRows a, const AttnPlan& p, int cache, bool paged, void* workspace, hipStream_t st) {
     const uint32_t dp = padded_dim(a.head_dim);
-    const uint32_t block = p.few ? kFewWaves * few_keys(dp, elem_bytes(cache)) : tile_keys_of(dp);
-    a.block_shift = uint32_t(__builtin_ctz(block));
-    XP_CHECK(p.few ? launch_few(a, cache, p.items, st) : launch_tile(a, cache, paged, p.items, st));
-    if (p.target == 0) return XP_OK;
-    const dim3 grid(a.n_tokens * a.heads);
-    if (dp == 64) hipLaunchKernelGGL((rows_attn_join_kernel<64>), grid, dim3(kJoinThreads), 0, st, a);
-    else if (dp == 128) hipLaunchKernelGGL((rows_attn_join_kernel<128>), grid, dim3(kJoinThreads), 0, st, a);
-    else hipLaunchKernelGGL((rows_attn_join_kernel<256>), grid, dim3(kJoinThreads), 0, st, a);
+    set_group(a);
+    a.row_shift = p.row_shift;
+    a.block_shift = uint32_t(__builtin_ctz(p.few ? kFewWaves * few_keys(dp, elem_bytes(cache)) : tile_keys_of(dp)));
+    // what the list may hold, and 32-bit places in it
+    const uint64_t most = uint64_t(p.tiles) * ((uint64_t(a.most_keys) >> a.block_shift) + 4);
+    a.target = workspace && most < 0x7FFFFFFFull ? p.target : 0u;
+    a.target_shift = a.target ? uint32_t(__builtin_ctz(a.target)) : 0u;
+    a.most_blocks = uint32_t(std::min<uint64_t>(most, 0x7FFFFFFFu));
+    a.part = static_cast<float*>(workspace);
+    const uint32_t grid = a.target ? a.target : p.tiles;
+    XP_CHECK(p.few ? launch_few(a, cache, grid, st) : launch_tile(a, cache, paged, grid, st));
+    if (a.target == 0) return XP_OK;
+    const dim3 join(kJoinSlices, a.target), block(kJoinThreads);
+    if (dp == 64) hipLaunchKernelGGL((rows_attn_join_kernel<64>), join, block, 0, st, a);
+    else if (dp == 128) hipLaunchKernelGGL((rows_attn_join_kernel<128>), join, block, 0, st, a);
+    else hipLaunchKernelGGL((rows_attn_join_kernel<256>), join, block, 0, st, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return set_error(XP_E_HIP, "%s: kernel launch -> %s", fn, hipGetErrorString(e));
     return XP_OK;
 }
@@ -163,6 +187,7 @@ int xp_attention_paged(const xp_rows* out, const xp_rows* q, const xp_paged_kv* 
     a.q_stride = q->stride, a.out_stride = out->stride;
     a.cu = s->cu, a.kv_len = s->kv_len, a.map = page_map(c, s), a.n_seq = s->n_seq, a.n_tokens = s->n_tokens;
     a.heads = q->heads, a.kv_heads = c->kv_heads, a.head_dim = c->head_dim, a.window = window, a.q_elem = q->elem, a.scale = scale;
+    a.most_keys = int32_t(std::min<uint64_t>(uint64_t(s->table) * c->page_size, kMostKeys));
     return attention_call(__func__, a, attn_plan(true, a.n_tokens, a.n_seq, a.heads, a.kv_heads, a.head_dim), c->elem, true, workspace,
                           as_stream(stream));
 }
@@ -185,6 +210,7 @@ int xp_attention_packed(const xp_rows* out, const xp_rows* q, const xp_rows* k, 
     a.q_stride = q->stride, a.k_stride = k->stride, a.v_stride = v->stride, a.out_stride = out->stride;
     a.cu = cu, a.n_seq = n_seq, a.n_tokens = n_tokens;
     a.heads = q->heads, a.kv_heads = k->heads, a.head_dim = head_dim, a.window = window, a.q_elem = q->elem, a.scale = scale;
+    a.most_keys = int32_t(std::min<uint32_t>(n_tokens, kMostKeys));
     return attention_call(__func__, a, attn_plan(false, n_tokens, n_seq, a.heads, a.kv_heads, head_dim), k->elem, false, workspace,
                           as_stream(stream));
 }

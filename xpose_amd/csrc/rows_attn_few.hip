@@ -27,7 +27,7 @@ struct FewTile {
     };
 };
 
-template <int CACHE, int DP, int TERMS>
+template <int CACHE, int DP, int TERMS, bool LIST>
 __global__ __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) void rows_attn_few_kernel(AttnRows a) {
     using T = FewTile<CACHE, DP>;
     constexpr int SZ = T::SZ, RB = T::RB, NC = T::NC, RPI = T::RPI, KT = T::KT, KG = KT / 16;
@@ -39,77 +39,86 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) void rows_attn_few_
     __shared__ Stage s1[kFewWaves];
     __shared__ float2 s_ml[kFewWaves][kFewRows];
 
-    const Item it = deal_item(a, blockIdx.x);
-    if (!it.live) return;
     const uint32_t lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t n16 = lane % 16, g = lane / 16, group = a.heads / a.kv_heads;
-    const TileSeq ts = tile_seq(a, it.seq);
-    const uint32_t n_rows = ts.n_new * group;
-    const int32_t past = ts.past;
+    const uint32_t rowbytes = a.head_dim * SZ, pmask = (1u << a.map.page_shift) - 1u;
+
+    __shared__ UnitsLds s_units;
+    Dealer<LIST> deal(a, s_units);
+    SeqWork sw{};
+    if (LIST) deal.join(a, Piece{}, sw, 0);
+    for (Piece it = deal.next(a, &sw); it.live; it = deal.next(a, &sw)) {
+    const uint32_t n_rows = sw.n_new * group, first = sw.first;
+    const int32_t past = sw.past;
     const uint32_t r0 = it.tile * kFewRows, r1 = min(r0 + kFewRows, n_rows);
-    const uint32_t row = min(r0 + n16, r1 - 1u), tok = row / group, head = it.kv_head * group + row % group;
-    const int32_t pos0 = past + int32_t(r0 / group), pos1 = past + int32_t((r1 - 1u) / group);   // of the tile's first and last row
-    const TileKeys keys = tile_keys(a, pos0, pos1, it.part, it.chunk);
+    const uint32_t row = min(r0 + n16, r1 - 1u), tok = by_group(a, row), head = it.kv_head * group + (row - tok * group);
+    const int32_t pos0 = past + int32_t(by_group(a, r0)), pos1 = past + int32_t(by_group(a, r1 - 1u));   // of the tile's first and last row
+    const KeyRange keys = seen_keys(a, pos0, pos1);
     // the positions that this lane's row sees, and those that all of the tile's do
     const int32_t back = a.window && a.window <= uint32_t(kMostKeys) ? int32_t(a.window) - 1 : kMostKeys;
-    const int32_t see1 = past + int32_t(tok), see0 = see1 - back, all0 = pos1 - back, all1 = pos0;
+    const int32_t see1 = past + int32_t(tok), see0 = min(see1 - back, a.most_keys), all0 = pos1 - back, all1 = pos0;
 
     // K's chunk of a step: 16 bytes, eight dims of 16 bits, or two runs of eight of 8 bits
-    u32x4 qh[QS], ql[TERMS == 2 ? QS : 1];
-    const float up = load_query<BF16, TERMS, QS, 4>(qh, ql, a, uint64_t(ts.first + tok) * a.q_stride + uint64_t(head) * a.head_dim, [&](int s) {
-        return SZ == 2 ? uint32_t(32 * s) + 8u * g : uint32_t(64 * (s / 2)) + 16u * g + 8u * (s % 2);
-    });
-    const float coef = a.scale * 1.4426950408889634f * up;
+    auto dim = [&](int s) { return SZ == 2 ? uint32_t(32 * s) + 8u * g : uint32_t(64 * (s / 2)) + 16u * g + 8u * (s % 2); };
+    Query<BF16, TERMS, QS, 4> q;
+    q.read(a, uint64_t(first + tok) * a.q_stride + uint64_t(head) * a.head_dim, dim);
 
-    const uint32_t rowbytes = a.head_dim * SZ;
-    const uint32_t pmask = (1u << a.map.page_shift) - 1u;
-    // the loads of keys [key0, key0 + KT) into a stage; the pages that have no rows come back as a mask of groups of 16
-    auto issue = [&](int32_t key0, Stage& s) -> uint32_t {
+    constexpr int32_t STEP = kFewWaves * KT;
+    const int32_t n = int32_t(it.n), k0 = (keys.lo / STEP + int32_t(it.blk)) * STEP + int32_t(wave) * KT;
+    // the pages of steps i .. i + 63, a lane each
+    int32_t lane_pages[KG];
+    auto read_pages = [&](int32_t i) {
+#pragma unroll
+        for (int x = 0; x < KG; ++x) lane_pages[x] = lane_page(a, it.seq, keys, k0 + (i + int32_t(lane)) * STEP + 16 * x);
+    };
+    // the loads of step i into a stage; the groups of 16 keys that have no page come back as a mask
+    auto issue = [&](int32_t i, Stage& s) -> uint32_t {
+        const int32_t key0 = k0 + i * STEP;
         int32_t page[KG];
         uint32_t bad = 0;
+        bool whole = key0 >= keys.lo && key0 + KT <= keys.hi && rowbytes == uint32_t(RB);
+        if (i != 0 && i % 64 == 0) read_pages(i);
 #pragma unroll
         for (int x = 0; x < KG; ++x) {
-            const int32_t k = key0 + 16 * x;
-            const bool in = k < keys.hi && k + 16 > keys.lo;
-            page[x] = in ? uniform_page(a.map, it.seq, k) : -1;
-            if (in && page[x] < 0) bad |= 1u << x;
+            page[x] = __builtin_amdgcn_readlane(lane_pages[x], i % 64);
+            if (page[x] == kNoPage) bad |= 1u << x;
+            whole = whole && page[x] >= 0;
         }
-        const bool whole = key0 >= keys.lo && key0 + KT <= keys.hi && bad == 0 && rowbytes == uint32_t(RB);
         const uint32_t kl = lds_offset(s.k), vl = lds_offset(s.v), off = (lane / NC) * rowbytes;
         const void* zero = &g_attn_zero;
         auto each = [&](auto put) {
 #pragma unroll
-            for (int i = 0; i < T::LOADS; ++i) {
-                const uint32_t rt = uint32_t(i * RPI) + lane / NC;         // this lane's key of the tile
+            for (int j = 0; j < T::LOADS; ++j) {
+                const uint32_t rt = uint32_t(j * RPI) + lane / NC;         // this lane's key of the tile
                 const uint32_t ck = 16u * ((lane % NC) ^ swizzle_k<NC>(rt)), cv = 16u * ((lane % NC) ^ swizzle_v<NC, SZ == 1, 4>(rt));
-                const int32_t pg = page[i * RPI / 16];
-                const uint64_t base = cache_row(uint32_t(max(pg, 0)), a.kv_heads, it.kv_head, a.map.page_shift, (uint32_t(key0) + i * RPI) & pmask) * rowbytes;
-                put(i, rt, ck, cv, pg, static_cast<const unsigned char*>(a.k) + base, static_cast<const unsigned char*>(a.v) + base);
+                const int32_t pg = page[j * RPI / 16];
+                const uint64_t base = cache_row(uint32_t(max(pg, 0)), a.kv_heads, it.kv_head, a.map.page_shift, (uint32_t(key0) + j * RPI) & pmask) * rowbytes;
+                put(j, rt, ck, cv, pg, static_cast<const unsigned char*>(a.k) + base, static_cast<const unsigned char*>(a.v) + base);
             }
         };
         if (whole)
-            each([&](int i, uint32_t, uint32_t ck, uint32_t cv, int32_t, const unsigned char* kb, const unsigned char* vb) {
-                to_lds16(kb, off + ck, kl + i * 1024);
-                to_lds16(vb, off + cv, vl + i * 1024);
+            each([&](int j, uint32_t, uint32_t ck, uint32_t cv, int32_t, const unsigned char* kb, const unsigned char* vb) {
+                to_lds16<true>(kb, off + ck, kl + j * 1024);
+                to_lds16<true>(vb, off + cv, vl + j * 1024);
             });
         else
-            each([&](int i, uint32_t rt, uint32_t ck, uint32_t cv, int32_t pg, const unsigned char* kb, const unsigned char* vb) {
+            each([&](int j, uint32_t rt, uint32_t ck, uint32_t cv, int32_t pg, const unsigned char* kb, const unsigned char* vb) {
                 const int32_t k = key0 + int32_t(rt);
                 const bool in = k >= keys.lo && k < keys.hi && pg >= 0;
-                to_lds16(in && ck < rowbytes ? kb + (off + ck) : zero, kl + i * 1024);
-                to_lds16(in && cv < rowbytes ? vb + (off + cv) : zero, vl + i * 1024);
+                to_lds16<true>(in && ck < rowbytes ? kb + (off + ck) : zero, kl + j * 1024);
+                to_lds16<true>(in && cv < rowbytes ? vb + (off + cv) : zero, vl + j * 1024);
             });
         if constexpr (SZ == 1) {
             const uint32_t sl = lds_offset(s.scale);
 #pragma unroll
-            for (int i = 0; i < T::SCALES; ++i) {
-                const uint32_t j = i * 64 + lane, kt = j % KT;             // K's KT scales, then V's
+            for (int y = 0; y < T::SCALES; ++y) {
+                const uint32_t j = y * 64 + lane, kt = j % KT;             // K's KT scales, then V's
                 int32_t p = page[0];
 #pragma unroll
                 for (int x = 1; x < KG; ++x) p = kt / 16 == uint32_t(x) ? page[x] : p;
                 const int32_t k = key0 + int32_t(kt);
                 const float* sp = (j < KT ? a.k_scale : a.v_scale) + cache_row(uint32_t(max(p, 0)), a.kv_heads, it.kv_head, a.map.page_shift, uint32_t(k) & pmask);
-                to_lds4(p >= 0 && k >= keys.lo && k < keys.hi ? static_cast<const void*>(sp) : zero, sl + i * 256);
+                to_lds4(p >= 0 && k >= keys.lo && k < keys.hi ? static_cast<const void*>(sp) : zero, sl + y * 256);
             }
         }
         return bad;
@@ -120,7 +129,7 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) void rows_attn_few_
     for (int t = 0; t < OT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f, ref = 0.0f, rl = -100.0f;   // ref: what the sums are relative to, m and the scales' exponent
 
-    auto work = [&](int32_t key0, const Stage& s, uint32_t bad) {
+    auto work = [&](int32_t key0, const Stage& s, uint32_t bad, float coef) {
         if (key0 >= keys.hi || key0 + KT <= keys.lo) return;
         const uint32_t fk = swizzle_k<NC>(n16);
         float sc[KG][4];
@@ -133,8 +142,8 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) void rows_attn_few_
 #pragma unroll
                 for (int st = 0; st < QS; ++st) {
                     const u32x4 kf = *reinterpret_cast<const u32x4*>(kr + 16 * ((4 * st + g) ^ f));
-                    if constexpr (TERMS == 2) c = mfma16<BF16>(kf, ql[st], c);
-                    c = mfma16<BF16>(kf, qh[st], c);
+                    if constexpr (TERMS == 2) c = mfma16<BF16>(kf, q.lo[st], c);
+                    c = mfma16<BF16>(kf, q.hi[st], c);
                 }
             } else {
 #pragma unroll
@@ -144,8 +153,8 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) void rows_attn_few_
                     for (int y = 0; y < 2; ++y) {
                         const u32x2 k0 = widen4<CACHE>(kb[2 * y]), k1 = widen4<CACHE>(kb[2 * y + 1]);
                         const u32x4 kf{k0[0], k0[1], k1[0], k1[1]};
-                        if constexpr (TERMS == 2) c = mfma16<BF16>(kf, ql[st + y], c);
-                        c = mfma16<BF16>(kf, qh[st + y], c);
+                        if constexpr (TERMS == 2) c = mfma16<BF16>(kf, q.lo[st + y], c);
+                        c = mfma16<BF16>(kf, q.hi[st + y], c);
                     }
                 }
             }
@@ -231,29 +240,26 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) void rows_attn_few_
     };
 
     // two stages: the loads of one are on their way while the other is worked on
-    constexpr int32_t STEP = kFewWaves * KT;
-    const int32_t n = keys.end - keys.first, k0 = keys.first * STEP + int32_t(wave) * KT;
-    if (n > 0) {
-        uint32_t bad0 = issue(k0, s0[wave]), bad1 = 0;
-        for (int32_t i = 0; i < n; i += 2) {
-            if (i + 1 < n) {
-                bad1 = issue(k0 + (i + 1) * STEP, s1[wave]);
-                wait_loads<T::OPS>();
-            } else {
-                wait_loads<0>();
-            }
-            work(k0 + i * STEP, s0[wave], bad0);
-            if (i + 1 >= n) break;
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (i + 2 < n) {
-                bad0 = issue(k0 + (i + 2) * STEP, s0[wave]);
-                wait_loads<T::OPS>();
-            } else {
-                wait_loads<0>();
-            }
-            work(k0 + (i + 1) * STEP, s1[wave], bad1);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    read_pages(0);
+    uint32_t bad0 = issue(0, s0[wave]), bad1 = 0;
+    if (1 < n) bad1 = issue(1, s1[wave]);
+    q.take(a, dim);
+    const float coef = a.scale * 1.4426950408889634f * q.up;
+    for (int32_t i = 0; i < n; i += 2) {
+        if (i + 1 < n) wait_loads<T::OPS>();
+        else wait_loads<0>();
+        work(k0 + i * STEP, s0[wave], bad0, coef);
+        if (i + 1 >= n) break;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (i + 2 < n) {
+            bad0 = issue(i + 2, s0[wave]);
+            wait_loads<T::OPS>();
+        } else {
+            wait_loads<0>();
         }
+        work(k0 + (i + 1) * STEP, s1[wave], bad1, coef);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (i + 3 < n) bad1 = issue(i + 3, s1[wave]);
     }
 
     // the waves' sums, relative to the largest reference
@@ -285,25 +291,28 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) void rows_attn_few_
             for (int j = 0; j < 4; ++j) o[j] += ml.x == -INFINITY ? 0.0f : x[j] * f;
         }
         if (d >= a.head_dim) continue;
-        if (a.target) {
-            float* part = a.part + uint64_t(blockIdx.x) * uint64_t(part_floats(kFewRows, DP));
+        if (LIST && it.n < it.of) {
+            float* part = part_record(a, deal.wg, it.blk == 0, part_floats(kFewRows, DP));
             *reinterpret_cast<f32x4*>(part + r * DP + d) = o;
             if (d == 0) reinterpret_cast<float2*>(part + kFewRows * DP)[r] = {top, sum};
             continue;
         }
-        const uint32_t rr = r0 + r, t = rr / group;
+        const uint32_t rr = r0 + r, t = by_group(a, rr);
         if (past + int32_t(t) < 0) continue;
-        store_row4(a, ts.first + t, it.kv_head * group + rr % group, d, o, sum);
+        store_row4(a, first + t, it.kv_head * group + (rr - t * group), d, o, sum);
+    }
+    if (LIST && it.blk == 0 && it.n < it.of) deal.join(a, it, sw, r1 - r0);
+    __syncthreads();                                   // the stages are the next piece's
     }
 }
 
-template <int CACHE, int TERMS>
-int launch_dim(const AttnRows& a, uint32_t items, hipStream_t st) {
-    const dim3 grid(items), block(kFewThreads);
+template <int CACHE, int TERMS, bool LIST>
+int launch_dim(const AttnRows& a, uint32_t grid_size, hipStream_t st) {
+    const dim3 grid(grid_size), block(kFewThreads);
     switch (padded_dim(a.head_dim)) {
-        case 64: hipLaunchKernelGGL((rows_attn_few_kernel<CACHE, 64, TERMS>), grid, block, 0, st, a); break;
-        case 128: hipLaunchKernelGGL((rows_attn_few_kernel<CACHE, 128, TERMS>), grid, block, 0, st, a); break;
-        default: hipLaunchKernelGGL((rows_attn_few_kernel<CACHE, 256, TERMS>), grid, block, 0, st, a); break;
+        case 64: hipLaunchKernelGGL((rows_attn_few_kernel<CACHE, 64, TERMS, LIST>), grid, block, 0, st, a); break;
+        case 128: hipLaunchKernelGGL((rows_attn_few_kernel<CACHE, 128, TERMS, LIST>), grid, block, 0, st, a); break;
+        default: hipLaunchKernelGGL((rows_attn_few_kernel<CACHE, 256, TERMS, LIST>), grid, block, 0, st, a); break;
     }
     XP_LAUNCHED();
     return XP_OK;
@@ -311,14 +320,18 @@ int launch_dim(const AttnRows& a, uint32_t items, hipStream_t st) {
 
 }  // namespace
 
-int launch_few(const AttnRows& a, int cache, uint32_t items, hipStream_t st) {
+template <bool LIST>
+static int launch_list(const AttnRows& a, int cache, uint32_t grid_size, hipStream_t st) {
     const bool two = a.q_elem == XP_ELEM_F32;
     switch (cache) {
-        case XP_ELEM_BF16: return launch_dim<XP_ELEM_BF16, 1>(a, items, st);
-        case XP_ELEM_F16: return two ? launch_dim<XP_ELEM_F16, 2>(a, items, st) : launch_dim<XP_ELEM_F16, 1>(a, items, st);
-        case XP_ELEM_I8: return two ? launch_dim<XP_ELEM_I8, 2>(a, items, st) : launch_dim<XP_ELEM_I8, 1>(a, items, st);
-        default: return two ? launch_dim<XP_ELEM_E4M3, 2>(a, items, st) : launch_dim<XP_ELEM_E4M3, 1>(a, items, st);
+        case XP_ELEM_BF16: return launch_dim<XP_ELEM_BF16, 1, LIST>(a, grid_size, st);
+        case XP_ELEM_F16: return two ? launch_dim<XP_ELEM_F16, 2, LIST>(a, grid_size, st) : launch_dim<XP_ELEM_F16, 1, LIST>(a, grid_size, st);
+        case XP_ELEM_I8: return two ? launch_dim<XP_ELEM_I8, 2, LIST>(a, grid_size, st) : launch_dim<XP_ELEM_I8, 1, LIST>(a, grid_size, st);
+        default: return two ? launch_dim<XP_ELEM_E4M3, 2, LIST>(a, grid_size, st) : launch_dim<XP_ELEM_E4M3, 1, LIST>(a, grid_size, st);
     }
+}
+int launch_few(const AttnRows& a, int cache, uint32_t grid_size, hipStream_t st) {
+    return a.target ? launch_list<true>(a, cache, grid_size, st) : launch_list<false>(a, cache, grid_size, st);
 }
 
 }  // namespace xp

@@ -25,7 +25,7 @@ struct KeyTile {
     };
 };
 
-template <int CACHE, int DP, int TERMS, bool PAGED>
+template <int CACHE, int DP, int TERMS, bool PAGED, bool LIST>
 __global__ __launch_bounds__(kTileThreads, DP == 256 || TERMS == 2 ? 1 : 2) void rows_attn_tile_kernel(AttnRows a) {
     using T = KeyTile<CACHE, DP>;
     constexpr int SZ = T::SZ, RB = T::RB, NC = T::NC, RPI = T::RPI, KT = T::KT, KG = KT / 32;
@@ -38,77 +38,85 @@ __global__ __launch_bounds__(kTileThreads, DP == 256 || TERMS == 2 ? 1 : 2) void
     __shared__ Stage s1;
     __shared__ uint32_t s_bad[2][KT / 32];       // keys of a tile whose V row is not finite
 
-    const Item it = deal_item(a, blockIdx.x);
-    if (!it.live) return;
     const uint32_t lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
     const uint32_t n32 = lane % 32, h = lane / 32, group = a.heads / a.kv_heads;
-    const TileSeq ts = tile_seq(a, it.seq);
-    const uint32_t n_rows = ts.n_new * group;
-    const int32_t past = ts.past;
+    const uint32_t rowbytes = a.head_dim * SZ, pmask = (1u << a.map.page_shift) - 1u;
+
+    __shared__ UnitsLds s_units;
+    Dealer<LIST> deal(a, s_units);
+    SeqWork sw{};
+    if (LIST) deal.join(a, Piece{}, sw, 0);
+    for (Piece it = deal.next(a, &sw); it.live; it = deal.next(a, &sw)) {
+    const uint32_t n_rows = sw.n_new * group, first = sw.first;
+    const int32_t past = sw.past;
     const uint32_t r0 = it.tile * kTileRows, r1 = min(r0 + kTileRows, n_rows);
     const uint32_t wr0 = r0 + 32 * wave;                                   // this wave's rows
     const bool idle = wr0 >= r1;
-    const uint32_t wr1 = min(wr0 + 32, r1);
-    const uint32_t row = idle ? r1 - 1u : min(wr0 + n32, wr1 - 1u), tok = row / group, head = it.kv_head * group + row % group;
-    const TileKeys keys = tile_keys(a, past + int32_t(r0 / group), past + int32_t((r1 - 1u) / group), it.part, it.chunk);
+    const uint32_t wr1 = min(wr0 + 32, r1), wa = idle ? r1 - 1u : wr0, wb = idle ? r1 - 1u : wr1 - 1u;
+    const uint32_t row = min(wa + n32, wb), tok = by_group(a, row), head = it.kv_head * group + (row - tok * group);
+    // of the tile's first and last row, and of the wave's
+    const int32_t tp0 = past + int32_t(by_group(a, r0)), tp1 = past + int32_t(by_group(a, r1 - 1u));
+    const int32_t p0 = past + int32_t(by_group(a, wa)), p1 = past + int32_t(by_group(a, wb));
+    const KeyRange keys = seen_keys(a, tp0, tp1);
     const int32_t back = a.window && a.window <= uint32_t(kMostKeys) ? int32_t(a.window) - 1 : kMostKeys;
-    const int32_t see1 = past + int32_t(tok), see0 = see1 - back;
+    const int32_t see1 = past + int32_t(tok), see0 = min(see1 - back, a.most_keys);
     // the positions that all of the wave's rows see, and that any does
-    const int32_t p0 = past + int32_t(uniform(idle ? r1 - 1u : wr0) / group), p1 = past + int32_t((idle ? r1 - 1u : wr1 - 1u) / group);
-    const int32_t all0 = p1 - back, all1 = p0, any0 = p0 - back, any1 = p1;
+    const int32_t all0 = p1 - back, all1 = p0, any0 = min(p0 - back, a.most_keys), any1 = p1;
 
-    u32x4 qh[QS], ql[TERMS == 2 ? QS : 1];
-    const float up = load_query<BF16, TERMS, QS, 2>(qh, ql, a, uint64_t(ts.first + tok) * a.q_stride + uint64_t(head) * a.head_dim, [&](int s) {
-        return SZ == 2 ? uint32_t(16 * s) + 8u * h : uint32_t(32 * (s / 2)) + 16u * h + 8u * (s % 2);
-    });
-    const float coef = a.scale * 1.4426950408889634f * up;
+    auto dim = [&](int s) { return SZ == 2 ? uint32_t(16 * s) + 8u * h : uint32_t(32 * (s / 2)) + 16u * h + 8u * (s % 2); };
+    Query<BF16, TERMS, QS, 2> q;
+    q.read(a, uint64_t(first + tok) * a.q_stride + uint64_t(head) * a.head_dim, dim);
 
-    const uint32_t rowbytes = a.head_dim * SZ;
-    const uint32_t pmask = (1u << a.map.page_shift) - 1u;
-    auto issue = [&](int32_t key0, Stage& s) -> uint32_t {
-        uint32_t bad = 0;                                                  // groups of 16 keys without a page
+    const int32_t n = int32_t(it.n), k0 = (keys.lo / KT + int32_t(it.blk)) * KT;
+    // the pages of the 64 groups of 16 keys from step i on, a lane each, and those of the steps after
+    constexpr int GROUPS = KT / 16, AHEAD = 64 / GROUPS;
+    int32_t lane_pages = kNoKeys, next_pages = kNoKeys;
+    uint64_t no_page = 0, no_row = 0;
+    auto read_pages = [&](int32_t i) { return lane_page(a, it.seq, keys, k0 + i * KT + 16 * int32_t(lane)); };
+    auto set_pages = [&](int32_t pages) {
+        lane_pages = pages;
+        no_page = __ballot(pages == kNoPage);
+        no_row = __ballot(pages < 0);
+    };
+    // the loads of step i into a stage; the groups of 16 keys that have no page come back as a mask
+    auto issue = [&](int32_t i, Stage& s) -> uint32_t {
+        const int32_t key0 = k0 + i * KT;
         const uint32_t kl = lds_offset(s.k), vl = lds_offset(s.v);
         const bool inside = key0 >= keys.lo && key0 + KT <= keys.hi;
+        const void* zero = &g_attn_zero;
+        uint32_t bad = 0;
         if constexpr (PAGED) {
-            int32_t page[KT / 16];
-#pragma unroll
-            for (int x = 0; x < KT / 16; ++x) {
-                const int32_t k = key0 + 16 * x;
-                const bool in = k < keys.hi && k + 16 > keys.lo;
-                page[x] = in ? uniform_page(a.map, it.seq, k) : -1;
-                if (in && page[x] < 0) bad |= 1u << x;
+            if (i != 0 && i % AHEAD == 0) {
+                set_pages(next_pages);
+                if (i + AHEAD < n) next_pages = read_pages(i + AHEAD);
             }
-            const bool whole = inside && bad == 0 && rowbytes == uint32_t(RB);
+            const uint32_t at = uint32_t(i % AHEAD) * GROUPS;
+            bad = uint32_t(no_page >> at) & ((1u << GROUPS) - 1u);
+            const bool whole = inside && (uint32_t(no_row >> at) & ((1u << GROUPS) - 1u)) == 0u && rowbytes == uint32_t(RB);
             const uint32_t off = (lane / NC) * rowbytes;
 #pragma unroll
-            for (int i = 0; i < T::LOADS; ++i) {
-                const uint32_t ri = (uint32_t(i) * kTileWaves + wave) * RPI, rt = ri + lane / NC;
+            for (int j = 0; j < T::LOADS; ++j) {
+                const uint32_t ri = (uint32_t(j) * kTileWaves + wave) * RPI, rt = ri + lane / NC;
                 const uint32_t ck = 16u * ((lane % NC) ^ swizzle_k<NC>(rt)), cv = 16u * ((lane % NC) ^ swizzle_v<NC, SZ == 1, 3>(rt));
-                int32_t pg = page[0];
-#pragma unroll
-                for (int x = 1; x < KT / 16; ++x) pg = ri / 16 == uint32_t(x) ? page[x] : pg;
+                const int32_t pg = __builtin_amdgcn_readlane(lane_pages, int(at + ri / 16));
                 const uint64_t base = cache_row(uint32_t(max(pg, 0)), a.kv_heads, it.kv_head, a.map.page_shift, (uint32_t(key0) + ri) & pmask) * rowbytes;
                 const unsigned char *kb = static_cast<const unsigned char*>(a.k) + base, *vb = static_cast<const unsigned char*>(a.v) + base;
                 if (whole) {
-                    to_lds16(kb, off + ck, kl + ri * RB);
-                    to_lds16(vb, off + cv, vl + ri * RB);
+                    to_lds16<false>(kb, off + ck, kl + ri * RB);
+                    to_lds16<false>(vb, off + cv, vl + ri * RB);
                 } else {
                     const int32_t k = key0 + int32_t(rt);
                     const bool in = k >= keys.lo && k < keys.hi && pg >= 0;
-                    const void* zero = &g_attn_zero;
-                    to_lds16(in && ck < rowbytes ? kb + (off + ck) : zero, kl + ri * RB);
-                    to_lds16(in && cv < rowbytes ? vb + (off + cv) : zero, vl + ri * RB);
+                    to_lds16<false>(in && ck < rowbytes ? kb + (off + ck) : zero, kl + ri * RB);
+                    to_lds16<false>(in && cv < rowbytes ? vb + (off + cv) : zero, vl + ri * RB);
                 }
             }
             if constexpr (SZ == 1) {
                 // wave 0: K's scales, wave 1: V's
                 if (wave < 2) {
-                    int32_t p = page[0];
-#pragma unroll
-                    for (int x = 1; x < KT / 16; ++x) p = (lane % KT) / 16 == uint32_t(x) ? page[x] : p;
-                    const int32_t k = key0 + int32_t(lane % KT);
+                    const int32_t p = __shfl(lane_pages, int(at + (lane % KT) / 16), kWave), k = key0 + int32_t(lane % KT);
                     const float* sp = (wave == 0 ? a.k_scale : a.v_scale) + cache_row(uint32_t(max(p, 0)), a.kv_heads, it.kv_head, a.map.page_shift, uint32_t(k) & pmask);
-                    const void* from = p >= 0 && k >= keys.lo && k < keys.hi ? static_cast<const void*>(sp) : &g_attn_zero;
+                    const void* from = p >= 0 && k >= keys.lo && k < keys.hi ? static_cast<const void*>(sp) : zero;
                     if (KT == 64 || lane < uint32_t(KT)) to_lds4(from, lds_offset(s.scale) + wave * KT * 4);
                 }
             }
@@ -116,15 +124,14 @@ __global__ __launch_bounds__(kTileThreads, DP == 256 || TERMS == 2 ? 1 : 2) void
             const uint32_t head_at = it.kv_head * rowbytes;
             const uint64_t kst = a.k_stride * SZ, vst = a.v_stride * SZ;
 #pragma unroll
-            for (int i = 0; i < T::LOADS; ++i) {
-                const uint32_t ri = (uint32_t(i) * kTileWaves + wave) * RPI, rt = ri + lane / NC;
+            for (int j = 0; j < T::LOADS; ++j) {
+                const uint32_t ri = (uint32_t(j) * kTileWaves + wave) * RPI, rt = ri + lane / NC;
                 const uint32_t ck = 16u * ((lane % NC) ^ swizzle_k<NC>(rt)), cv = 16u * ((lane % NC) ^ swizzle_v<NC, SZ == 1, 3>(rt));
                 const int32_t k = key0 + int32_t(rt);
                 const bool in = inside || (k >= keys.lo && k < keys.hi);
-                const uint64_t tk = uint64_t(ts.first) + uint64_t(k);
-                const void* zero = &g_attn_zero;
-                to_lds16(in && ck < rowbytes ? static_cast<const unsigned char*>(a.k) + tk * kst + (head_at + ck) : zero, kl + ri * RB);
-                to_lds16(in && cv < rowbytes ? static_cast<const unsigned char*>(a.v) + tk * vst + (head_at + cv) : zero, vl + ri * RB);
+                const uint64_t tk = uint64_t(first) + uint64_t(k);
+                to_lds16<false>(in && ck < rowbytes ? static_cast<const unsigned char*>(a.k) + tk * kst + (head_at + ck) : zero, kl + ri * RB);
+                to_lds16<false>(in && cv < rowbytes ? static_cast<const unsigned char*>(a.v) + tk * vst + (head_at + cv) : zero, vl + ri * RB);
             }
         }
         return bad;
@@ -165,7 +172,7 @@ __global__ __launch_bounds__(kTileThreads, DP == 256 || TERMS == 2 ? 1 : 2) void
         }
     };
 
-    auto work = [&](int32_t key0, Stage& s, uint32_t bad, const uint32_t* flags) {
+    auto work = [&](int32_t key0, Stage& s, uint32_t bad, const uint32_t* flags, float coef) {
         if (idle || key0 > any1 || key0 + KT <= any0) return;
         const uint32_t fk = swizzle_k<NC>(n32);
         f32x16 sc[KG];
@@ -178,8 +185,8 @@ __global__ __launch_bounds__(kTileThreads, DP == 256 || TERMS == 2 ? 1 : 2) void
 #pragma unroll
                 for (int st = 0; st < QS; ++st) {
                     const u32x4 kf = *reinterpret_cast<const u32x4*>(kr + 16 * ((2 * st + h) ^ fk));
-                    if constexpr (TERMS == 2) sc[x] = mfma32<BF16>(kf, ql[st], sc[x]);
-                    sc[x] = mfma32<BF16>(kf, qh[st], sc[x]);
+                    if constexpr (TERMS == 2) sc[x] = mfma32<BF16>(kf, q.lo[st], sc[x]);
+                    sc[x] = mfma32<BF16>(kf, q.hi[st], sc[x]);
                 }
             } else {
 #pragma unroll
@@ -189,8 +196,8 @@ __global__ __launch_bounds__(kTileThreads, DP == 256 || TERMS == 2 ? 1 : 2) void
                     for (int y = 0; y < 2; ++y) {
                         const u32x2 k0 = widen4<CACHE>(kb[2 * y]), k1 = widen4<CACHE>(kb[2 * y + 1]);
                         const u32x4 kf{k0[0], k0[1], k1[0], k1[1]};
-                        if constexpr (TERMS == 2) sc[x] = mfma32<BF16>(kf, ql[st + y], sc[x]);
-                        sc[x] = mfma32<BF16>(kf, qh[st + y], sc[x]);
+                        if constexpr (TERMS == 2) sc[x] = mfma32<BF16>(kf, q.lo[st + y], sc[x]);
+                        sc[x] = mfma32<BF16>(kf, q.hi[st + y], sc[x]);
                     }
                 }
                 // keys 8 i + 4 h + 0..3 of the 32
@@ -298,10 +305,10 @@ __global__ __launch_bounds__(kTileThreads, DP == 256 || TERMS == 2 ? 1 : 2) void
                     const bool sees = k >= see0 && k <= see1;
                     uint64_t at;
                     if constexpr (PAGED) {
-                        const int32_t pg = uniform_page(a.map, it.seq, k);
+                        const int32_t pg = uniform_page(a.map, it.seq, k);   // it has one: a row without is zeros
                         at = cache_row(uint32_t(max(pg, 0)), a.kv_heads, it.kv_head, a.map.page_shift, uint32_t(k) & pmask) * a.head_dim;
                     } else {
-                        at = (uint64_t(ts.first) + uint64_t(k)) * a.v_stride + uint64_t(it.kv_head) * a.head_dim;
+                        at = (uint64_t(first) + uint64_t(k)) * a.v_stride + uint64_t(it.kv_head) * a.head_dim;
                     }
 #pragma unroll
                     for (int t = 0; t < OT; ++t)
@@ -320,36 +327,39 @@ __global__ __launch_bounds__(kTileThreads, DP == 256 || TERMS == 2 ? 1 : 2) void
         }
     };
 
-    // whether all of the tile's rows see all keys of a block
-    const int32_t tall0 = past + int32_t((r1 - 1u) / group) - back, tall1 = past + int32_t(r0 / group);
-    const int32_t n = keys.end - keys.first, k0 = keys.first * KT;
-    auto step = [&](int32_t i, Stage& cur, Stage& next, uint32_t bad, uint32_t* flags) -> uint32_t {
+    // the positions that all of the tile's rows see
+    const int32_t tall0 = tp1 - back, tall1 = tp0;
+    auto step = [&](int32_t i, Stage& cur, Stage& next, uint32_t bad, uint32_t* flags, float coef) -> uint32_t {
         const int32_t key0 = k0 + i * KT;
         wait_loads<0>();
         if (SZ == 2 && threadIdx.x < KT / 32) flags[threadIdx.x] = 0;
         __syncthreads();
         uint32_t nbad = 0;
-        if (i + 1 < n) nbad = issue(key0 + KT, next);
+        if (i + 1 < n) nbad = issue(i + 1, next);
         const bool part = SZ == 2 && (key0 < tall0 || key0 + KT - 1 > tall1);
         if (part) {
             sieve(cur, flags);
             __syncthreads();
         }
-        work(key0, cur, bad, part ? flags : nullptr);
+        work(key0, cur, bad, part ? flags : nullptr, coef);
         return nbad;
     };
-    if (n > 0) {
-        uint32_t bad = issue(k0, s0);
-        for (int32_t i = 0; i < n; i += 2) {
-            bad = step(i, s0, s1, bad, s_bad[0]);
-            if (i + 1 < n) bad = step(i + 1, s1, s0, bad, s_bad[1]);
-        }
+    if constexpr (PAGED) {
+        set_pages(read_pages(0));
+        if (AHEAD < n) next_pages = read_pages(AHEAD);
+    }
+    uint32_t bad = issue(0, s0);
+    q.take(a, dim);
+    const float coef = a.scale * 1.4426950408889634f * q.up;
+    for (int32_t i = 0; i < n; i += 2) {
+        bad = step(i, s0, s1, bad, s_bad[0], coef);
+        if (i + 1 < n) bad = step(i + 1, s1, s0, bad, s_bad[1], coef);
     }
 
     l += __shfl_xor(l, 32, kWave);
-    if (idle || wr0 + n32 >= r1) return;
-    if (a.target) {
-        float* part = a.part + uint64_t(blockIdx.x) * part_floats(kTileRows, DP);
+    const bool live = !idle && wr0 + n32 < r1;
+    if (LIST && live && it.n < it.of) {
+        float* part = part_record(a, deal.wg, it.blk == 0, part_floats(kTileRows, DP));
         const uint32_t r = row - r0;
 #pragma unroll
         for (int t = 0; t < OT; ++t)
@@ -357,25 +367,27 @@ __global__ __launch_bounds__(kTileThreads, DP == 256 || TERMS == 2 ? 1 : 2) void
             for (int j = 0; j < 4; ++j)
                 *reinterpret_cast<f32x4*>(part + r * DP + 32 * t + 8 * j + 4 * h) = f32x4{acc[t][4 * j], acc[t][4 * j + 1], acc[t][4 * j + 2], acc[t][4 * j + 3]};
         if (h == 0) reinterpret_cast<float2*>(part + kTileRows * DP)[r] = {m == -INFINITY && l == 0.0f ? -INFINITY : ref, l};
-        return;
+    } else if (live && see1 >= 0) {
+#pragma unroll
+        for (int t = 0; t < OT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t d = 32 * t + 8 * j + 4 * h;
+                if (d < a.head_dim) store_row4(a, first + tok, head, d, f32x4{acc[t][4 * j], acc[t][4 * j + 1], acc[t][4 * j + 2], acc[t][4 * j + 3]}, l);
+            }
     }
-    if (see1 < 0) return;
-#pragma unroll
-    for (int t = 0; t < OT; ++t)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t d = 32 * t + 8 * j + 4 * h;
-            if (d < a.head_dim) store_row4(a, ts.first + tok, head, d, f32x4{acc[t][4 * j], acc[t][4 * j + 1], acc[t][4 * j + 2], acc[t][4 * j + 3]}, l);
-        }
+    if (LIST && it.blk == 0 && it.n < it.of) deal.join(a, it, sw, r1 - r0);
+    __syncthreads();                                   // the stages are the next piece's
+    }
 }
 
-template <int CACHE, int TERMS, bool PAGED>
-int launch_dim(const AttnRows& a, uint32_t items, hipStream_t st) {
-    const dim3 grid(items), block(kTileThreads);
+template <int CACHE, int TERMS, bool PAGED, bool LIST>
+int launch_dim(const AttnRows& a, uint32_t grid_size, hipStream_t st) {
+    const dim3 grid(grid_size), block(kTileThreads);
     switch (padded_dim(a.head_dim)) {
-        case 64: hipLaunchKernelGGL((rows_attn_tile_kernel<CACHE, 64, TERMS, PAGED>), grid, block, 0, st, a); break;
-        case 128: hipLaunchKernelGGL((rows_attn_tile_kernel<CACHE, 128, TERMS, PAGED>), grid, block, 0, st, a); break;
-        default: hipLaunchKernelGGL((rows_attn_tile_kernel<CACHE, 256, TERMS, PAGED>), grid, block, 0, st, a); break;
+        case 64: hipLaunchKernelGGL((rows_attn_tile_kernel<CACHE, 64, TERMS, PAGED, LIST>), grid, block, 0, st, a); break;
+        case 128: hipLaunchKernelGGL((rows_attn_tile_kernel<CACHE, 128, TERMS, PAGED, LIST>), grid, block, 0, st, a); break;
+        default: hipLaunchKernelGGL((rows_attn_tile_kernel<CACHE, 256, TERMS, PAGED, LIST>), grid, block, 0, st, a); break;
     }
     XP_LAUNCHED();
     return XP_OK;
@@ -383,15 +395,20 @@ int launch_dim(const AttnRows& a, uint32_t items, hipStream_t st) {
 
 }  // namespace
 
-int launch_tile(const AttnRows& a, int cache, bool paged, uint32_t items, hipStream_t st) {
-    if (!paged) return cache == XP_ELEM_F16 ? launch_dim<XP_ELEM_F16, 1, false>(a, items, st) : launch_dim<XP_ELEM_BF16, 1, false>(a, items, st);
+template <bool LIST>
+static int launch_list(const AttnRows& a, int cache, bool paged, uint32_t grid_size, hipStream_t st) {
+    if (!paged)
+        return cache == XP_ELEM_F16 ? launch_dim<XP_ELEM_F16, 1, false, LIST>(a, grid_size, st) : launch_dim<XP_ELEM_BF16, 1, false, LIST>(a, grid_size, st);
     const bool two = a.q_elem == XP_ELEM_F32;
     switch (cache) {
-        case XP_ELEM_BF16: return launch_dim<XP_ELEM_BF16, 1, true>(a, items, st);
-        case XP_ELEM_F16: return two ? launch_dim<XP_ELEM_F16, 2, true>(a, items, st) : launch_dim<XP_ELEM_F16, 1, true>(a, items, st);
-        case XP_ELEM_I8: return two ? launch_dim<XP_ELEM_I8, 2, true>(a, items, st) : launch_dim<XP_ELEM_I8, 1, true>(a, items, st);
-        default: return two ? launch_dim<XP_ELEM_E4M3, 2, true>(a, items, st) : launch_dim<XP_ELEM_E4M3, 1, true>(a, items, st);
+        case XP_ELEM_BF16: return launch_dim<XP_ELEM_BF16, 1, true, LIST>(a, grid_size, st);
+        case XP_ELEM_F16: return two ? launch_dim<XP_ELEM_F16, 2, true, LIST>(a, grid_size, st) : launch_dim<XP_ELEM_F16, 1, true, LIST>(a, grid_size, st);
+        case XP_ELEM_I8: return two ? launch_dim<XP_ELEM_I8, 2, true, LIST>(a, grid_size, st) : launch_dim<XP_ELEM_I8, 1, true, LIST>(a, grid_size, st);
+        default: return two ? launch_dim<XP_ELEM_E4M3, 2, true, LIST>(a, grid_size, st) : launch_dim<XP_ELEM_E4M3, 1, true, LIST>(a, grid_size, st);
     }
+}
+int launch_tile(const AttnRows& a, int cache, bool paged, uint32_t grid_size, hipStream_t st) {
+    return a.target ? launch_list<true>(a, cache, paged, grid_size, st) : launch_list<false>(a, cache, paged, grid_size, st);
 }
 
 }  // namespace xp

@@ -1,65 +1,13 @@
 // What the kernels of attention over packed rows share (rows_attn_few.hip,
-// rows_attn_tile.hip, rows_attention.hip): arguments, how the work is dealt to
-// workgroups, operands of the matrix instructions, tiles on their way to LDS.
+// rows_attn_tile.hip, rows_attention.hip): their places in the deal, operands of
+// the matrix instructions, tiles on their way to LDS.
 #pragma once
 
 #include "xp_elem.hpp"
+#include "xp_rows_deal.hpp"
 
 namespace xp {
 
-struct AttnRows {
-    const void *q, *k, *v;         // k, v: the cache's planes, or the packed rows
-    void*       out;
-    const float *k_scale, *v_scale;
-    uint64_t    q_stride, k_stride, v_stride, out_stride;   // elements
-    const int32_t *cu, *kv_len;    // kv_len NULL: packed
-    PageMap     map;
-    uint32_t    n_seq, n_tokens, heads, kv_heads, head_dim, window;
-    int32_t     q_elem;
-    float       scale;
-    // The deal (deal_item): rows of a tile and keys of a block (powers of two),
-    // the items aimed at (0: the keys are not split), where the parts of split keys go
-    uint32_t    row_shift, block_shift, target, items;
-    float*      part;
-};
-
-// ---- how the work is dealt -------------------------------------------------------
-// Row i of sequence b and kv head h is token i / group, head h group + i %
-// group: the query heads of one kv head share its keys. An item is a tile of
-// tile_rows such rows with a run of `chunk` blocks of the keys that the tile
-// sees. Without a split there is one item a tile. With one, chunk is the same
-// for all tiles and makes about `target` items of the whole call: workgroups
-// with equal work, whatever the lengths. Every workgroup works that out from
-// the lengths itself (64 sequences a step of a wave), as does the kernel that
-// joins the parts. Items of a sequence run from its last tile, which sees the
-// most keys, to its first; the kv head changes fastest, so that the tiles of a
-// head meet in one XCD's L2 where kv_heads shares a factor with 8.
-struct SeqWork {
-    uint32_t tiles, span;          // row tiles of one kv head, most key blocks of any tile
-};
-constexpr int32_t kMostKeys = 1 << 30;      // of a sequence
-XP_HD SeqWork seq_work(const AttnRows& a, uint32_t b) {
-    const RowSpan r = row_span(a.cu, a.n_tokens, b);
-    const uint32_t n = r.end - r.first, group = a.heads / a.kv_heads;
-    int32_t len = a.kv_len ? a.kv_len[b] : int32_t(n);
-    len = len < 0 ? 0 : (len > kMostKeys ? kMostKeys : len);
-    uint32_t keys = uint32_t(len);
-    if (a.window) {
-        // the tokens of a tile's rows see a window before the first and
-        // themselves, from anywhere in a block on
-        const uint32_t seen = a.window > uint32_t(kMostKeys) ? uint32_t(kMostKeys) : a.window;
-        const uint32_t most = seen + ((1u << a.row_shift) - 1u) / group + 1u + (1u << a.block_shift);
-        keys = most < keys ? most : keys;
-    }
-    const uint32_t m = (1u << a.row_shift) - 1u, k = (1u << a.block_shift) - 1u;
-    return {(n * group + m) >> a.row_shift, (keys + k) >> a.block_shift};
-}
-XP_HD uint32_t parts_of(const SeqWork& w, uint32_t chunk) { return w.span <= chunk ? 1u : (w.span + chunk - 1) / chunk; }
-
-struct Item {
-    uint32_t seq, tile, part, kv_head, chunk;
-    bool     live;
-};
 #ifdef __HIPCC__
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
 __device__ __forceinline__ uint32_t of_lane(uint32_t v, uint32_t lane) { return uint32_t(__builtin_amdgcn_readlane(int(v), int(lane))); }
@@ -76,66 +24,136 @@ __device__ __forceinline__ uint32_t wave_scan_add(uint32_t v) {
     v = dpp_add<0x142, 0xA>(v);    // row_bcast:15 -> rows 1, 3
     return dpp_add<0x143, 0xC>(v); // row_bcast:31 -> rows 2, 3
 }
-// Blocks of a part, in a call of up to 64 sequences from w of each lane's (any
-// rounding of the sum is every wave's).
-__device__ __forceinline__ uint32_t chunk_of(const AttnRows& a, float blocks) {
-    if (a.target == 0) return 0x7FFFFFFFu;
-    return uniform(uint32_t(fminf(fmaxf(ceilf(blocks * float(a.kv_heads) / float(a.target)), 1.0f), 1e9f)));
-}
 __device__ __forceinline__ SeqWork lane_work(const AttnRows& a, uint32_t b) {
-    return b < a.n_seq ? seq_work(a, b) : SeqWork{0, 0};
+    return b < a.n_seq ? seq_work(a, b) : SeqWork{0, 0, 0, 0};
 }
-__device__ __forceinline__ uint32_t deal_chunk(const AttnRows& a) {
-    if (a.target == 0) return 0x7FFFFFFFu;
-    float blocks = 0.0f;
-    for (uint32_t b0 = 0; b0 < a.n_seq; b0 += kWave) {
-        const SeqWork w = lane_work(a, b0 + threadIdx.x % kWave);
-        blocks += float(w.tiles) * float(w.span);
+__device__ __forceinline__ SeqWork work_of_lane(const SeqWork& w, uint32_t l) {
+    return {of_lane(w.first, l), of_lane(w.n_new, l), of_lane(w.tiles, l), int32_t(of_lane(uint32_t(w.past), l))};
+}
+// The units (tiles, or with LIST blocks of the list, of all kv heads) of up to 64
+// sequences a lane each, and their sums up to and with each lane's. (The sums of a
+// cu that gives rows many times over may wrap: the callers bound what they find.)
+template <bool LIST>
+struct LaneUnits {
+    SeqWork  w;
+    uint32_t own, up;
+    __device__ __forceinline__ void read(const AttnRows& a, uint32_t b0) {
+        w = lane_work(a, b0 + threadIdx.x % kWave);
+        own = (LIST ? head_list(a, w).blocks : w.tiles) * a.kv_heads;
+        up = wave_scan_add(own);
     }
-    return chunk_of(a, wave_sum(blocks));
-}
-// Item i of the call; not live past the last one.
-__device__ __forceinline__ Item deal_item(const AttnRows& a, uint32_t i) {
-    const uint32_t lane = threadIdx.x % kWave;
-    SeqWork w = lane_work(a, lane);
-    // up to 64 sequences are read once
-    const uint32_t chunk = a.n_seq <= kWave ? chunk_of(a, wave_sum(float(w.tiles) * float(w.span))) : deal_chunk(a);
-    uint32_t before = 0;
-    for (uint32_t b0 = 0; b0 < a.n_seq; b0 += kWave) {
-        if (b0) w = lane_work(a, b0 + lane);
-        const uint32_t parts = parts_of(w, chunk), own = w.tiles * parts * a.kv_heads, up = wave_scan_add(own);
-        const uint64_t hit = __ballot(i < before + up);
-        if (hit) {
-            const uint32_t l = uint32_t(__ffsll(static_cast<long long>(hit))) - 1u;
-            const uint32_t np = of_lane(parts, l), nt = of_lane(w.tiles, l);
-            uint32_t j = i - before - of_lane(up - own, l);
-            const uint32_t h = j % a.kv_heads;
-            j /= a.kv_heads;
-            // (sums of a cu that gives rows many times over may have wrapped)
-            return {uniform(b0 + l), uniform(nt - 1u - j / np), uniform(j % np), uniform(h), chunk, j / np < nt};
+    __device__ __forceinline__ uint32_t all() const { return of_lane(up, kWave - 1); }
+};
+// The sequence that a unit is in, and the unit's place in it.
+struct Found {
+    SeqWork  w;
+    uint32_t seq, at;
+    bool     live;
+};
+// The call's units. The first 64 sequences' are kept in LDS, not in registers: every
+// wave writes them there, the same, and reads what it has written.
+struct UnitsLds {
+    uint32_t v[6][kWave];
+};
+template <bool LIST>
+struct Units {
+    UnitsLds& lds;
+    uint32_t  total;
+    __device__ __forceinline__ Units(const AttnRows& a, UnitsLds& s) : lds(s), total(0) {
+        const uint32_t lane = threadIdx.x % kWave;
+        LaneUnits<LIST> u;
+        u.read(a, 0);
+        s.v[0][lane] = u.w.n_new, s.v[1][lane] = u.w.tiles, s.v[2][lane] = uint32_t(u.w.past), s.v[3][lane] = u.own, s.v[4][lane] = u.up;
+        s.v[5][lane] = u.w.first;
+        total = u.all();
+        if (a.n_seq > kWave)
+            for (uint32_t b0 = kWave; b0 < a.n_seq; b0 += kWave) {
+                LaneUnits<LIST> v;
+                v.read(a, b0);
+                total += v.all();
+            }
+        if (LIST) total = min(total, a.most_blocks);
+    }
+    __device__ __forceinline__ Found find(const AttnRows& a, uint32_t i) const {
+        const uint32_t lane = threadIdx.x % kWave;
+        uint32_t before = 0;
+        LaneUnits<LIST> v{{lds.v[5][lane], lds.v[0][lane], lds.v[1][lane], int32_t(lds.v[2][lane])}, lds.v[3][lane], lds.v[4][lane]};
+        for (uint32_t b0 = 0; b0 < a.n_seq; b0 += kWave) {
+            if (b0) v.read(a, b0);
+            const uint64_t hit = __ballot(i < before + v.up);
+            if (hit) {
+                const uint32_t l = uint32_t(__ffsll(static_cast<long long>(hit))) - 1u;
+                return {work_of_lane(v.w, l), uniform(b0 + l), uniform(i - before - of_lane(v.up - v.own, l)), true};
+            }
+            before += v.all();
         }
-        before += of_lane(up, kWave - 1);
+        return {{0, 0, 0, 0}, 0, 0, false};
     }
-    return {0, 0, 0, 0, chunk, false};
+};
+// The piece at place `at` of the list (n up to the tile's end; 0: not live, or a
+// gap of `of`).
+__device__ __forceinline__ Piece list_piece(const AttnRows& a, const Units<true>& units, uint32_t at, SeqWork* work) {
+    const Found f = units.find(a, at);
+    Piece p{0, 0, 0, 0, 0, 0, false};
+    if (!f.live) return p;
+    const HeadList l = head_list(a, f.w);
+    const uint32_t h = l.blocks ? f.at / l.blocks : a.kv_heads;
+    if (h >= a.kv_heads) return p;
+    p = head_piece(a, f.w, l, f.at - h * l.blocks);
+    *work = f.w;
+    return {f.seq, uniform(p.tile), uniform(h), uniform(p.blk), uniform(p.n), uniform(p.of), p.live};
 }
-// The first item of tile `tile` of sequence `seq`, kv head `head`, and how many
-// parts it has; they follow each other kv_heads apart.
-__device__ __forceinline__ uint32_t deal_first(const AttnRows& a, uint32_t seq, uint32_t tile, uint32_t head, uint32_t* n_parts) {
-    const uint32_t lane = threadIdx.x % kWave, chunk = deal_chunk(a);
-    uint32_t before = 0;
-    for (uint32_t b0 = 0; b0 < a.n_seq; b0 += kWave) {
-        const SeqWork w = lane_work(a, b0 + lane);
-        const uint32_t parts = parts_of(w, chunk), own = w.tiles * parts * a.kv_heads, up = wave_scan_add(own);
-        if (seq < b0 + kWave) {
-            const uint32_t l = seq - b0;
-            *n_parts = of_lane(parts, l);
-            return before + of_lane(up - own, l) + (of_lane(w.tiles, l) - 1u - tile) * *n_parts * a.kv_heads + head;
+// Workgroup `block` of the grid as one of the list: neighbours in it share keys, so
+// each XCD (which takes every eighth workgroup) gets an eighth of it.
+__device__ __forceinline__ uint32_t list_wg(const AttnRows& a, uint32_t blocks, uint32_t block) {
+    return blocks > a.target && a.target % 8 == 0 ? (block % 8) * (a.target / 8) + block / 8 : block;
+}
+
+// The pieces of this workgroup, one after the other, with the sequence's work.
+template <bool LIST>
+struct Dealer {
+    Units<LIST> units;
+    uint32_t    at, end, wg;       // of the list
+    __device__ __forceinline__ Dealer(const AttnRows& a, UnitsLds& s) : units(a, s), at(0), end(1), wg(blockIdx.x) {
+        if constexpr (LIST) {
+            wg = uniform(list_wg(a, units.total, blockIdx.x));
+            at = uniform(wg < units.total ? run_first(a, units.total, wg) : 0u);
+            end = uniform(wg < units.total ? run_first(a, units.total, wg + 1) : 0u);
         }
-        before += of_lane(up, kWave - 1);
     }
-    *n_parts = 0;
-    return 0;
-}
+    // For the join: of the last piece that next() gave, or that there was none to join.
+    __device__ __forceinline__ void join(const AttnRows& a, const Piece& p, const SeqWork& w, uint32_t rows) const {
+        const uint32_t last = at - p.n - p.blk + p.of - 1u;       // the tile's last block
+        const uint32_t parts = p.live && p.blk == 0 && p.n < p.of && last < units.total ? run_of(a, units.total, last) - wg + 1u : 0u;
+        if (threadIdx.x == 0)
+            reinterpret_cast<JoinTile*>(a.part)[wg] = {parts, p.tile << a.row_shift, rows, p.kv_head, w.first, w.past, {0, 0}};
+    }
+    // (not live at the end)
+    __device__ __forceinline__ Piece next(const AttnRows& a, SeqWork* work) {
+        if constexpr (LIST) {
+            while (at < end) {
+                Piece p = list_piece(a, units, at, work);
+                if (!p.live) break;
+                if (p.n) {
+                    p.n = min(p.n, end - at);
+                    at += p.n;
+                    return p;
+                }
+                at += p.of;
+            }
+        } else if (at < end) {
+            at = end;
+            const Found f = units.find(a, blockIdx.x);
+            const uint32_t tile = f.w.tiles - 1u - f.at / a.kv_heads;
+            if (f.live && tile < f.w.tiles) {
+                *work = f.w;
+                const uint32_t n = tile_blocks(a, f.w, tile).n;
+                return {f.seq, uniform(tile), uniform(f.at % a.kv_heads), 0, uniform(n), uniform(n), n > 0};
+            }
+        }
+        return {0, 0, 0, 0, 0, 0, false};
+    }
+};
 
 // Uniform words of tables that no kernel changes while it runs.
 __device__ __forceinline__ int32_t uniform_word(const int32_t* p, uint64_t i) {
@@ -148,30 +166,14 @@ __device__ __forceinline__ int32_t uniform_page(const PageMap& m, uint32_t b, in
     return g >= 0 && uint32_t(g) < m.n_pages ? g : -1;
 }
 
-// A tile's sequence: its packed rows and the position of its first new token.
-struct TileSeq {
-    uint32_t first, n_new;
-    int32_t  past;                 // negative where it is shorter than its new rows
-};
-__device__ __forceinline__ TileSeq tile_seq(const AttnRows& a, uint32_t b) {
-    const int32_t n = int32_t(a.n_tokens);
-    const int32_t x = min(max(uniform_word(a.cu, b), 0), n), y = min(max(uniform_word(a.cu, b + 1), x), n);
-    const int32_t len = a.kv_len ? min(max(uniform_word(a.kv_len, b), 0), kMostKeys) : y - x;
-    return {uint32_t(x), uint32_t(y - x), len - (y - x)};
-}
-// The keys [lo, hi) that tokens at positions p0 .. p1 see, and of their blocks
-// the run [first, end) of one part.
-struct TileKeys {
-    int32_t lo, hi, first, end;
-};
-__device__ __forceinline__ TileKeys tile_keys(const AttnRows& a, int32_t p0, int32_t p1, uint32_t part, uint32_t chunk) {
-    TileKeys t;
-    t.hi = max(p1 + 1, 0);
-    t.lo = a.window && a.window <= uint32_t(kMostKeys) ? max(p0 - int32_t(a.window) + 1, 0) : 0;
-    const int32_t b0 = t.lo >> a.block_shift, b1 = (t.hi + (1 << a.block_shift) - 1) >> a.block_shift;
-    t.first = b0 + int32_t(part * chunk);
-    t.end = b1 - t.first > int32_t(chunk) ? t.first + int32_t(chunk) : b1;
-    return t;
+// The pages of the 16-key groups that lane l of a wave is asked for, in front of
+// their use: kNoKeys where no row of the tile sees the group, kNoPage where it has no
+// page.
+constexpr int32_t kNoKeys = -1, kNoPage = -2;
+__device__ __forceinline__ int32_t lane_page(const AttnRows& a, uint32_t seq, const KeyRange& keys, int32_t key) {
+    if (key >= keys.hi || key + 16 <= keys.lo) return kNoKeys;
+    const int32_t g = page_of(a.map, seq, key);
+    return g < 0 ? kNoPage : g;
 }
 
 // ---- operands ------------------------------------------------------------------------
@@ -249,7 +251,8 @@ __device__ __forceinline__ uint32_t swizzle_v(uint32_t key) {
 }
 
 // Loads straight into LDS, lane l's 16 (4) bytes to lds + 16 l (4 l): from a
-// lane's own address, or from an offset to a uniform one. In assembly, because the
+// lane's own address, or from an offset to a uniform one. ONCE marks them as not to be
+// kept in the caches (1 GiB read so: 7.0 TB/s, without 6.2). In assembly, because the
 // compiler puts a wait for every such load in flight before any read of LDS, the
 // other stage's too; the kernels wait themselves (wait_loads) before they read a
 // stage. No register is written, so nothing can be reused while they fly; the
@@ -258,11 +261,19 @@ __device__ __forceinline__ uint32_t swizzle_v(uint32_t key) {
 __device__ __forceinline__ uint32_t lds_offset(const void* p) {
     return uniform(uint32_t(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)p)));
 }
+template <bool ONCE>
 __device__ __forceinline__ void to_lds16(const void* from, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(uniform(lds)), "v"(from) : "memory", "m0");
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(uniform(lds)), "v"(from) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(uniform(lds)), "v"(from) : "memory", "m0");
 }
+template <bool ONCE>
 __device__ __forceinline__ void to_lds16(const void* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform(lds)), "v"(off), "s"(base) : "memory", "m0");
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(uniform(lds)), "v"(off), "s"(base) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(uniform(lds)), "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void to_lds4(const void* from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(uniform(lds)), "v"(from) : "memory", "m0");
@@ -316,57 +327,73 @@ __device__ __forceinline__ void two_terms(float x, float y, uint32_t& hi, uint32
 // head's dims: zeros). Queries of another type than the operands' (and those of
 // two terms) are taken as 2^e times F16 numbers, the row's largest in [2^14, 2^15),
 // so that none is out of range: BF16 ones keep all their bits down to 2^-38 of the
-// largest, and F32 ones are the sum of two terms, 21 bits. Returns 2^e. GROUPS: the
-// lanes that hold a row, 64 / GROUPS apart.
-template <bool BF16, int TERMS, int STEPS, int GROUPS, typename DimOf>
-__device__ __forceinline__ float load_query(u32x4 (&hi)[STEPS], u32x4 (&lo)[TERMS == 2 ? STEPS : 1], const AttnRows& a,
-                                            uint64_t at, DimOf dim) {
-    const uint32_t D = a.head_dim;
-    if (TERMS == 1 && a.q_elem == (BF16 ? XP_ELEM_BF16 : XP_ELEM_F16)) {
+// largest, and F32 ones are the sum of two terms, 21 bits. GROUPS: the lanes that
+// hold a row, 64 / GROUPS apart. read() only sends for them, so that the first keys'
+// loads are on their way before take() waits.
+template <bool BF16, int TERMS, int STEPS, int GROUPS>
+struct Query {
+    u32x4 hi[STEPS], lo[TERMS == 2 ? STEPS : 1];
+    float up;                      // 2^e
+    template <typename DimOf>
+    __device__ __forceinline__ void read(const AttnRows& a, uint64_t at, DimOf dim) {
+        const uint32_t D = a.head_dim;
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-        {
-            const bool in = dim(s) < D;
-            const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + (in ? at + dim(s) : at));
-            hi[s] = in ? w : u32x4{0u, 0u, 0u, 0u};
-        }
-        return 1.0f;
-    }
-    // (of two terms: F32 alone; of one: the other 16-bit type; dims past the
-    // head's: the row's first, as zeros)
-    float x[STEPS][8], top = 0.0f;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-        const bool in = dim(s) < D;
-        if constexpr (TERMS == 2) load8<XP_ELEM_F32>(a.q, in ? at + dim(s) : at, x[s]);
-        else load8<BF16 ? XP_ELEM_F16 : XP_ELEM_BF16>(a.q, in ? at + dim(s) : at, x[s]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[s][j] = in ? x[s][j] : 0.0f;
-            top = fmaxf(top, fabsf(x[s][j]));
-        }
-    }
-    top = max_xor32(top);
-    if constexpr (GROUPS == 4) top = max_xor16(top);
-    const uint32_t e = __float_as_uint(top) >> 23;
-    const bool fit = e >= 15u && e <= 253u;
-    const float down = fit ? __uint_as_float((268u - e) << 23) : 1.0f, up = fit ? __uint_as_float((e - 14u) << 23) : 1.0f;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float u = x[s][2 * w] * down, v = x[s][2 * w + 1] * down;
+        for (int s = 0; s < STEPS; ++s) {
+            const uint64_t i = dim(s) < D ? at + dim(s) : at;
             if constexpr (TERMS == 2) {
-                uint32_t p, r;
-                two_terms(u, v, p, r);
-                hi[s][w] = p;
-                lo[s][w] = r;
+                const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const float*>(a.q) + i);
+                hi[s] = p[0];
+                lo[s] = p[1];
             } else {
-                hi[s][w] = pack_op<BF16>(u, v);
+                hi[s] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + i);
             }
         }
-    return up;
-}
+    }
+    template <typename DimOf>
+    __device__ __forceinline__ void take(const AttnRows& a, DimOf dim) {
+        const uint32_t D = a.head_dim;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+            if (dim(s) >= D) {
+                hi[s] = u32x4{0u, 0u, 0u, 0u};
+                if constexpr (TERMS == 2) lo[s] = hi[s];
+            }
+        up = 1.0f;
+        if (TERMS == 1 && a.q_elem == (BF16 ? XP_ELEM_BF16 : XP_ELEM_F16)) return;
+        // F32, or the other 16-bit type
+        auto at = [&](int s, int j) -> float {
+            if constexpr (TERMS == 2) return __uint_as_float(j < 4 ? hi[s][j] : lo[s][j - 4]);
+            else if constexpr (BF16) return j % 2 ? f16_hi(hi[s][j / 2]) : f16_lo(hi[s][j / 2]);
+            else return j % 2 ? bf16hi(hi[s][j / 2]) : bf16lo(hi[s][j / 2]);
+        };
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(at(s, j)));
+        top = max_xor32(top);
+        if constexpr (GROUPS == 4) top = max_xor16(top);
+        const uint32_t e = __float_as_uint(top) >> 23;
+        const bool fit = e >= 15u && e <= 253u;
+        const float down = fit ? __uint_as_float((268u - e) << 23) : 1.0f;
+        up = fit ? __uint_as_float((e - 14u) << 23) : 1.0f;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            u32x4 h{}, r{};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float u = at(s, 2 * w) * down, v = at(s, 2 * w + 1) * down;
+                uint32_t p, q = 0;
+                if constexpr (TERMS == 2) two_terms(u, v, p, q);
+                else p = pack_op<BF16>(u, v);
+                h[w] = p;
+                r[w] = q;
+            }
+            hi[s] = h;
+            if constexpr (TERMS == 2) lo[s] = r;
+        }
+    }
+};
 
 // Four dims of an output row: o / sum, zeros where nothing was seen.
 __device__ __forceinline__ void store_row4(const AttnRows& a, uint32_t tok, uint32_t head, uint32_t d, f32x4 o, float sum) {
@@ -396,9 +423,14 @@ __device__ __forceinline__ float scale_exponent(float largest) {
 }
 #endif  // __HIPCC__
 
-// The parts of split keys: item i's rows, tile_rows sums of DP values each, then a
-// (maximum, sum) pair a row.
+// The parts: record 2 w + 1 of workgroup w for a tile that begins in its run and
+// does not end there, 2 w for one that began before. A record is tile_rows sums
+// of DP values, then a (reference, sum of weights) pair a row.
 XP_HD uint64_t part_floats(uint32_t tile_rows, uint32_t dp) { return uint64_t(tile_rows) * (dp + 2); }
+
+__device__ __forceinline__ float* part_record(const AttnRows& a, uint32_t wg, bool begins, uint64_t floats) {
+    return a.part + size_t(a.target) * (sizeof(JoinTile) / 4) + (2ull * wg + (begins ? 1u : 0u)) * floats;
+}
 
 inline uint32_t padded_dim(uint32_t d) { return d <= 64 ? 64u : d <= 128 ? 128u : 256u; }
 
@@ -409,8 +441,8 @@ XP_HD constexpr uint32_t few_keys(uint32_t dp, uint32_t size) {    // of a wave 
 }
 constexpr uint32_t kTileWaves = 4, kTileRows = 32 * kTileWaves;
 XP_HD constexpr uint32_t tile_keys_of(uint32_t dp) { return dp == 256 ? 32u : 64u; }
-// Launchers; `items` workgroups.
-int launch_few(const AttnRows& a, int cache, uint32_t items, hipStream_t st);
-int launch_tile(const AttnRows& a, int cache, bool paged, uint32_t items, hipStream_t st);
+// Launchers; `grid` workgroups.
+int launch_few(const AttnRows& a, int cache, uint32_t grid, hipStream_t st);
+int launch_tile(const AttnRows& a, int cache, bool paged, uint32_t grid, hipStream_t st);
 
 }  // namespace xp
