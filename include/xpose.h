@@ -374,8 +374,8 @@ enum xp_elem { XP_ELEM_F32 = 0, XP_ELEM_F16 = 1, XP_ELEM_BF16 = 2, XP_ELEM_I8 = 
 
 /* Rows of heads: token t's head h at data + (t stride + h head_dim) elements.
  * elem is F32, F16 or BF16; data 16-byte aligned and stride a multiple of 16
- * bytes and at least heads * head_dim (a larger one steps over what a fused
- * product leaves between). */
+ * bytes, at least heads * head_dim and at most 2^26 elements (a larger one than
+ * the heads steps over what a fused product leaves between). */
 typedef struct {
     void*    data;
     uint64_t stride;

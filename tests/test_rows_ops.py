@@ -121,7 +121,7 @@ def rows_args(xh, **kw):
 
 @pytest.mark.parametrize("bad,says", [
     ({"data": None}, "q is null"), ({"elem": 3}, "elem 3"), ({"heads": 0}, "heads"), ({"stride": 511}, "stride"),
-    ({"data": FAKE + 1}, "multiples of 2"), ({"stride": 1 << 33}, "2\\^32"), ({"heads": 4, "stride": 256}, "q_out has not")])
+    ({"data": FAKE + 1}, "multiples of 2"), ({"stride": 1 << 27}, "2\\^26"), ({"heads": 4, "stride": 256}, "q_out has not")])
 def test_rope_refuses_rows(xh, bad, says):
     with pytest.raises(xh.XposeError, match=says):
         xh.call("xp_rope_rows", rows_args(xh), rows_args(xh, **bad), None, None, FAKE, 4, 64, rope_spec(xh), None)

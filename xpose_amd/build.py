@@ -36,7 +36,7 @@ LIB_SOURCES = ["runtime.cpp", "synth.cpp", "matvec.hip", "transformer.hip", "sam
                "sampling_chain.hip", "token_kernel.hip", "probe.hip", "batch_kernels.hip", "batch_step.hip",
                "batch.cpp", "prefill_engine.hip", "prefill.cpp", "gguf.cpp", "pack.cpp", "tokenizer.cpp", "repack.cpp", "native_quant.hip", "prefill_kernels.hip",
                "session_kernels.hip", "session.cpp",
-               "rows.cpp", "rope_rows.hip", "paged_kv.hip", "rows_attention.hip", "rows_attn_few.hip", "rows_attn_tile.hip"]
+               "rows.cpp", "rope_rows.hip", "paged_kv.hip", "rows_attention.hip", "rows_attn_few.hip", "rows_attn_mid.hip", "rows_attn_tile.hip"]
 
 
 def _run(cmd: list[str], verbose: bool) -> None:

@@ -1,8 +1,12 @@
 // Rows into and out of a paged cache, quantised where it has 8 bits.
 //
-// A row (one token's k or v of one kv head) is taken by the least power of two
-// of lanes that hold it at eight elements each; its largest absolute value is
-// found by exchanges among them. Bytes bound both directions.
+// Bytes bound both directions. A workgroup takes a few tokens, all their heads' k and
+// v rows. A row is taken by the least power of two of lanes that hold it at eight elements
+// each (its largest absolute value is found by exchanges among them), kKvAhead
+// rows at a time, so that each lane has that many loads in flight; where the tokens'
+// rows lie in the cache is found meanwhile, a lane a token, and passed through LDS.
+// 32000 rows of 4 heads of 64 in f16, written and read back: 37.2 us a row at a time, KVA
+// so; 4300 of 8 heads of 128 from bf16 to e4m3 and back 26.6, KVB.
 #include <algorithm>
 
 #include "xp_elem.hpp"
@@ -11,6 +15,7 @@ namespace xp {
 namespace {
 
 constexpr uint32_t kKvThreads = 256;
+constexpr uint32_t kKvAhead = 4, kKvTokens = 64, kKvSeqs = 255;
 
 struct KvRows {
     void *         cache[2];       // k, v
@@ -19,20 +24,46 @@ struct KvRows {
     uint64_t       stride[2];
     const int32_t *cu, *kv_len;
     PageMap        map;
-    uint32_t       n_seq, n_tokens, kv_heads, head_dim, lanes;
+    uint32_t       n_seq, n_tokens, kv_heads, head_dim, lanes, tokens;
 };
 
-// The row of the cache that belongs to packed token t's head h: its index in
-// rows of head_dim, or -1 (no row); `owned` says whether a sequence has t.
-__device__ __forceinline__ int64_t row_in_cache(const KvRows& a, uint32_t t, uint32_t h, bool* owned) {
-    const uint32_t b = seq_of_row(a.cu, a.n_seq, a.n_tokens, t);
-    *owned = b < a.n_seq;
-    if (!*owned) return -1;
-    const RowSpan r = row_span(a.cu, a.n_tokens, b);
-    const int64_t p = row_position(a.kv_len[b], r.end - r.first, t - r.first);
-    *owned = p >= 0;
-    const int32_t g = page_of(a.map, b, p);
-    return g < 0 ? -1 : int64_t(cache_row(uint32_t(g), a.kv_heads, h, a.map.page_shift, uint32_t(p) & ((1u << a.map.page_shift) - 1u)));
+// Where the workgroup's tokens lie: the index of head 0's row in the cache, kNoRow
+// where the position has none, kNoSeq where the token belongs to no sequence.
+constexpr int64_t kNoRow = -1, kNoSeq = -2;
+struct KvSlots {
+    int32_t cu[kKvSeqs + 1];
+    int64_t at[kKvTokens];
+};
+__device__ __forceinline__ void find_slots(const KvRows& a, KvSlots& s, uint32_t t0) {
+    const bool few = a.n_seq <= kKvSeqs;
+    if (few && threadIdx.x <= a.n_seq) s.cu[threadIdx.x] = a.cu[threadIdx.x];
+    __syncthreads();
+    if (threadIdx.x < a.tokens) {
+        const uint32_t t = t0 + threadIdx.x;
+        int64_t at = kNoSeq;
+        if (t < a.n_tokens) {
+            const int32_t* cu = few ? s.cu : a.cu;
+            const uint32_t b = seq_of_row(cu, a.n_seq, a.n_tokens, t);
+            if (b < a.n_seq) {
+                const RowSpan r = row_span(cu, a.n_tokens, b);
+                const int64_t p = row_position(a.kv_len[b], r.end - r.first, t - r.first);
+                if (p >= 0) {
+                    const int32_t g = page_of(a.map, b, p);
+                    at = g < 0 ? kNoRow : int64_t(cache_row(uint32_t(g), a.kv_heads, 0, a.map.page_shift, uint32_t(p) & ((1u << a.map.page_shift) - 1u)));
+                }
+            }
+        }
+        s.at[threadIdx.x] = at;
+    }
+    __syncthreads();
+}
+// Row i of the workgroup's: its token (of them), plane and head.
+struct KvRow {
+    uint32_t token, kv, head;
+};
+__device__ __forceinline__ KvRow row_of(const KvRows& a, uint32_t i) {
+    const uint32_t t = i / (2u * a.kv_heads), w = i - t * 2u * a.kv_heads, kv = w >= a.kv_heads ? 1u : 0u;
+    return {t, kv, w - kv * a.kv_heads};
 }
 
 // x / scale rounded to the nearest whole number, even on a tie, of the exact
@@ -46,83 +77,101 @@ __device__ __forceinline__ int quantise1(float x, float scale, float inv) {
     return int(fminf(fmaxf(q, -127.0f), 127.0f));
 }
 
+// The scale and the eight codes of a row, from the largest of its absolute values'
+// bit patterns (as which an infinity is over every number and a NaN over it).
+template <int CACHE>
+__device__ __forceinline__ float quantise8(const float (&x)[8], uint32_t top, u32x2& code) {
+    code = u32x2{0u, 0u};
+    if (top >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
+    if (top == 0u) return 0.0f;
+    if constexpr (CACHE == XP_ELEM_I8) {
+        // at least the least normal number, whose reciprocal is finite
+        const float scale = fmaxf(__uint_as_float(top) / 127.0f, 0x1p-126f), inv = 1.0f / scale;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) code[j / 4] |= uint32_t(quantise1(x[j], scale, inv) & 0xFF) << (8 * (j % 4));
+        return scale;
+    } else {
+        // max <= 448 2^k = 1.75 2^(8 + k)
+        const int k = max(int(top >> 23) - 135 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0), -126);
+        const float inv = __uint_as_float(uint32_t(127 - k) << 23);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j] * inv, x[4 * j + 1] * inv, 0, false);
+            c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * inv, x[4 * j + 3] * inv, c, true);
+            code[j] = uint32_t(c);
+        }
+        return __uint_as_float(uint32_t(k + 127) << 23);
+    }
+}
+
 template <int IN, int CACHE>
 __global__ __launch_bounds__(kKvThreads) void paged_kv_write_kernel(KvRows a) {
+    __shared__ KvSlots slots;
     const uint32_t per = kKvThreads / a.lanes, sub = threadIdx.x / a.lanes, lane = threadIdx.x % a.lanes;
-    const uint64_t n = uint64_t(a.n_tokens) * a.kv_heads * 2;
+    const uint32_t t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.n_tokens - t0), n = nt * a.kv_heads * 2;
     const bool live = lane * 8 < a.head_dim;
-    for (uint64_t i0 = uint64_t(blockIdx.x) * per; i0 < n; i0 += uint64_t(gridDim.x) * per) {
-        const uint64_t i = i0 + sub;
-        const bool in = i < n;
-        const uint32_t t = uint32_t(in ? i / (a.kv_heads * 2) : 0), w = uint32_t(in ? i % (a.kv_heads * 2) : 0);
-        const uint32_t kv = w / a.kv_heads, h = w % a.kv_heads;
-        bool owned;
-        const int64_t row = in ? row_in_cache(a, t, h, &owned) : -1;
-        float x[8] = {};
-        if (row >= 0 && live) load8<IN>(a.rows[kv], uint64_t(t) * a.stride[kv] + uint64_t(h) * a.head_dim + lane * 8, x);
-        const uint64_t to = uint64_t(row) * a.head_dim + lane * 8;
-        if constexpr (CACHE == XP_ELEM_F16 || CACHE == XP_ELEM_BF16) {
-            if (row >= 0 && live) store8<CACHE>(a.cache[kv], to, x);
-        } else {
-            // as bit patterns an infinity is over every number and a NaN over it
-            uint32_t top = 0;
+    for (uint32_t i0 = 0; i0 < n; i0 += per * kKvAhead) {
+        float x[kKvAhead][8];
+        KvRow r[kKvAhead];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-            for (uint32_t o = 1; o < a.lanes; o <<= 1) top = max(top, uint32_t(__shfl_xor(int(top), int(o), kWave)));
-            const bool finite = top < 0x7F800000u;
-            float scale = 0.0f;
-            u32x2 code{0u, 0u};
-            if (!finite) {
-                scale = __uint_as_float(0x7FC00000u);
-            } else if (top != 0u) {
-                if constexpr (CACHE == XP_ELEM_I8) {
-                    // at least the least normal number, whose reciprocal is finite
-                    scale = fmaxf(__uint_as_float(top) / 127.0f, 0x1p-126f);
-                    const float inv = 1.0f / scale;
+        for (uint32_t j = 0; j < kKvAhead; ++j) {
+            const uint32_t i = i0 + j * per + sub;
+            r[j] = row_of(a, min(i, n - 1u));
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) code[j / 4] |= uint32_t(quantise1(x[j], scale, inv) & 0xFF) << (8 * (j % 4));
-                } else {
-                    // max <= 448 2^k = 1.75 2^(8 + k)
-                    const int k = max(int(top >> 23) - 135 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0), -126);
-                    scale = __uint_as_float(uint32_t(k + 127) << 23);
-                    const float inv = __uint_as_float(uint32_t(127 - k) << 23);
+            for (int e = 0; e < 8; ++e) x[j][e] = 0.0f;
+            if (i < n && live)
+                load8<IN>(a.rows[r[j].kv], uint64_t(t0 + r[j].token) * a.stride[r[j].kv] + uint64_t(r[j].head) * a.head_dim + lane * 8, x[j]);
+        }
+        if (i0 == 0) find_slots(a, slots, t0);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j] * inv, x[4 * j + 1] * inv, 0, false);
-                        c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * inv, x[4 * j + 3] * inv, c, true);
-                        code[j] = uint32_t(c);
-                    }
-                }
+        for (uint32_t j = 0; j < kKvAhead; ++j) {
+            const int64_t base = slots.at[r[j].token], row = base + (int64_t(r[j].head) << a.map.page_shift);
+            const bool put = base >= 0 && i0 + j * per + sub < n;
+            const uint64_t to = uint64_t(row) * a.head_dim + lane * 8;
+            if constexpr (CACHE == XP_ELEM_F16 || CACHE == XP_ELEM_BF16) {
+                if (put && live) store8<CACHE>(a.cache[r[j].kv], to, x[j]);
+            } else {
+                uint32_t top = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[j][e]) & 0x7FFFFFFFu);
+                for (uint32_t o = 1; o < a.lanes; o <<= 1) top = max(top, uint32_t(__shfl_xor(int(top), int(o), kWave)));
+                u32x2 code;
+                const float scale = quantise8<CACHE>(x[j], top, code);
+                if (put && live) *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.cache[r[j].kv]) + to) = code;
+                if (put && lane == 0) a.scale[r[j].kv][row] = scale;
             }
-            if (row >= 0 && live) *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.cache[kv]) + to) = code;
-            if (row >= 0 && lane == 0) a.scale[kv][row] = scale;
         }
     }
 }
 
 template <int OUT, int CACHE>
 __global__ __launch_bounds__(kKvThreads) void paged_kv_read_kernel(KvRows a) {
+    __shared__ KvSlots slots;
     const uint32_t per = kKvThreads / a.lanes, sub = threadIdx.x / a.lanes, lane = threadIdx.x % a.lanes;
-    const uint64_t n = uint64_t(a.n_tokens) * a.kv_heads * 2;
+    const uint32_t t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.n_tokens - t0), n = nt * a.kv_heads * 2;
+    find_slots(a, slots, t0);
     if (lane * 8 >= a.head_dim) return;
-    for (uint64_t i = uint64_t(blockIdx.x) * per + sub; i < n; i += uint64_t(gridDim.x) * per) {
-        const uint32_t t = uint32_t(i / (a.kv_heads * 2)), w = uint32_t(i % (a.kv_heads * 2));
-        const uint32_t kv = w / a.kv_heads, h = w % a.kv_heads;
-        bool owned;
-        const int64_t row = row_in_cache(a, t, h, &owned);
-        if (!owned) continue;
-        float x[8];
+    for (uint32_t i0 = 0; i0 < n; i0 += per * kKvAhead) {
+        float x[kKvAhead][8], s[kKvAhead];
+        KvRow r[kKvAhead];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __uint_as_float(0x7FC00000u);
-        if (row >= 0) {
-            load8<CACHE>(a.cache[kv], uint64_t(row) * a.head_dim + lane * 8, x);
-            if constexpr (CACHE == XP_ELEM_I8 || CACHE == XP_ELEM_E4M3) {
-                const float s = a.scale[kv][row];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= s;
+        for (uint32_t j = 0; j < kKvAhead; ++j) {
+            r[j] = row_of(a, min(i0 + j * per + sub, n - 1u));
+            const int64_t base = slots.at[r[j].token], row = max(base, int64_t(0)) + (int64_t(r[j].head) << a.map.page_shift);
+            s[j] = 1.0f;
+            if (base >= 0) {
+                load8<CACHE>(a.cache[r[j].kv], uint64_t(row) * a.head_dim + lane * 8, x[j]);
+                if constexpr (CACHE == XP_ELEM_I8 || CACHE == XP_ELEM_E4M3) s[j] = a.scale[r[j].kv][row];
             }
         }
-        store8<OUT>(a.rows[kv], uint64_t(t) * a.stride[kv] + uint64_t(h) * a.head_dim + lane * 8, x);
+#pragma unroll
+        for (uint32_t j = 0; j < kKvAhead; ++j) {
+            const int64_t base = slots.at[r[j].token];
+            if (i0 + j * per + sub >= n || base == kNoSeq) continue;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[j][e] = base < 0 ? __uint_as_float(0x7FC00000u) : CACHE == XP_ELEM_I8 || CACHE == XP_ELEM_E4M3 ? x[j][e] * s[j] : x[j][e];
+            store8<OUT>(a.rows[r[j].kv], uint64_t(t0 + r[j].token) * a.stride[r[j].kv] + uint64_t(r[j].head) * a.head_dim + lane * 8, x[j]);
+        }
     }
 }
 
@@ -140,10 +189,14 @@ int kv_call(const char* fn, const xp_paged_kv* c, const xp_paged_seqs* s, const 
     if (*skip) return XP_OK;
     XP_CHECK(check_here(fn, stream, out));
     *a = {{c->k, c->v}, {c->k_scale, c->v_scale}, {k->data, v->data}, {k->stride, v->stride}, s->cu, s->kv_len,
-          page_map(c, s), s->n_seq, s->n_tokens, c->kv_heads, c->head_dim, 1};
+          page_map(c, s), s->n_seq, s->n_tokens, c->kv_heads, c->head_dim, 1, 1};
     while (a->lanes * 8 < c->head_dim) a->lanes *= 2;
-    const uint64_t rows = uint64_t(s->n_tokens) * c->kv_heads * 2, per = kKvThreads / a->lanes;
-    *grid = dim3(uint32_t(std::min<uint64_t>((rows + per - 1) / per, 1u << 20)));
+    // tokens of a workgroup: as many as fill its loads once, and no fewer than 1024 workgroups
+    const uint32_t at_once = kKvAhead * (kKvThreads / a->lanes) / (2 * c->kv_heads);
+    a->tokens = std::max(1u, std::min({at_once, kKvTokens, s->n_tokens / 1024 + 1}));
+    const uint32_t groups = (s->n_tokens + a->tokens - 1) / a->tokens;
+    if (groups >= 1u << 24) return set_error(XP_E_ARG, "%s: %u tokens are over 2^24 workgroups", fn, s->n_tokens);
+    *grid = dim3(groups);
     return XP_OK;
 }
 

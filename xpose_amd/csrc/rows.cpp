@@ -11,7 +11,7 @@ int check_rows(const char* fn, const char* what, const xp_rows* r, uint32_t head
     if (r->stride < uint64_t(r->heads) * head_dim)
         return set_error(XP_E_ARG, "%s: %s: stride %llu is less than %u heads of %u", fn, what,
                          static_cast<unsigned long long>(r->stride), r->heads, head_dim);
-    if (r->stride > (1ull << 32)) return set_error(XP_E_ARG, "%s: %s: stride is over 2^32 elements", fn, what);
+    if (r->stride > (1ull << 26)) return set_error(XP_E_ARG, "%s: %s: stride is over 2^26 elements", fn, what);
     const uint32_t size = elem_bytes(r->elem);
     if (align < size) align = size;
     if (reinterpret_cast<uintptr_t>(r->data) % align || r->stride * size % align)

@@ -9,35 +9,62 @@
 // (rows_attn_few.hip) and for many (rows_attn_tile.hip). Where the rows alone
 // leave CUs without work the keys are split, and a second kernel joins the parts.
 #include <algorithm>
+#include <cmath>
 
 #include "xp_rows_attn.hpp"
 
 namespace xp {
 namespace {
 
-constexpr uint32_t kJoinThreads = 256, kJoinWaves = kJoinThreads / kWave;
-constexpr uint32_t kJoinSlices = 4;        // workgroups a tile
-constexpr int kJoinBatch = 16;             // parts that a wave reads at once
+constexpr uint32_t kJoinThreads = 256, kJoinWaves = kJoinThreads / kWave, kJoinGrid = 1024;
+constexpr uint32_t kMostTarget = 512;
+constexpr int kJoinBatch = 8;              // parts that a wave reads at once
 
-// Workgroup (slice, w) joins the tile that begins in run w and ends behind it, if
-// there is one: every kJoinSlices-th row: a wave a row, or, of few rows of many parts,
-// all four waves, every fourth part each.
+// The rows of all tiles that more than one workgroup worked on, shared out evenly: a
+// workgroup a row where there are no more rows than that, each wave every fourth part;
+// else a wave a row.
 template <int DP>
 __global__ __launch_bounds__(kJoinThreads) void rows_attn_join_kernel(AttnRows a) {
-    constexpr int PER = DP / kWave;
+    constexpr int PER = DP / kWave, TW = kMostTarget / kJoinThreads;
     typedef float vec __attribute__((ext_vector_type(PER)));
     __shared__ float s_o[kJoinWaves][DP];
     __shared__ float2 s_ml[kJoinWaves];
-    const uint32_t lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave), w0 = blockIdx.y;
-    const JoinTile p = reinterpret_cast<const JoinTile*>(a.part)[w0];
-    const uint32_t n = uniform(p.parts), r0 = p.r0, rows = uniform(p.rows), group = a.heads / a.kv_heads;
-    if (n < 2) return;
+    __shared__ uint32_t s_up[kMostTarget], s_sum[kJoinWaves];
+    const uint32_t lane = threadIdx.x % kWave, wave = uniform(threadIdx.x / kWave);
+    const JoinTile* tiles = reinterpret_cast<const JoinTile*>(a.part);
+    // the rows up to and with each workgroup's tile
+    uint32_t mine[TW], sum = 0;
+#pragma unroll
+    for (int j = 0; j < TW; ++j) {
+        const uint32_t w = threadIdx.x * TW + j;
+        mine[j] = w < a.target && tiles[w].parts > 1u ? tiles[w].rows : 0u;
+        sum += mine[j];
+    }
+    const uint32_t up = wave_scan_add(sum);
+    if (lane == kWave - 1) s_sum[wave] = up;
+    __syncthreads();
+    uint32_t before = up - sum, total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kJoinWaves; ++w) {
+        before += w < wave ? s_sum[w] : 0u;
+        total += s_sum[w];
+    }
+#pragma unroll
+    for (int j = 0; j < TW; ++j) s_up[threadIdx.x * TW + j] = before += mine[j];
+    __syncthreads();
+    total = uniform(total);
+    const bool all = total <= kJoinGrid;
+    const uint32_t group = a.heads / a.kv_heads, step = all ? kJoinWaves : 1u, at = all ? wave : 0u;
     const uint64_t size = part_floats(1u << a.row_shift, DP);
-    const float* base = part_record(a, w0, false, size);
-    const bool all = n >= 2 * kJoinWaves && rows <= kJoinWaves * kJoinSlices;     // all waves a row
-    const uint32_t step = all ? kJoinWaves : 1u, at = all ? wave : 0u;
-    for (uint32_t r = blockIdx.x + (all ? 0u : wave * kJoinSlices); r < rows; r += kJoinSlices * (all ? 1u : kJoinWaves)) {
-        const uint32_t t = by_group(a, r0 + r), head = p.kv_head * group + (r0 + r - t * group);
+    for (uint32_t i = all ? blockIdx.x : blockIdx.x * kJoinWaves + wave; i < total; i += kJoinGrid * (all ? 1u : kJoinWaves)) {
+        uint32_t w0 = 0;                   // the first tile whose sum is over i
+#pragma unroll
+        for (uint32_t s = kMostTarget / 2; s > 0; s /= 2) w0 += s_up[w0 + s - 1u] <= i ? s : 0u;
+        w0 = uniform(w0);
+        const JoinTile p = tiles[w0];
+        const uint32_t n = uniform(p.parts), r = uniform(i - (s_up[w0] - p.rows));
+        const uint32_t t = by_group(a, p.r0 + r), head = p.kv_head * group + (p.r0 + r - t * group);
+        const float* base = part_record(a, w0, false, size);
         float top = -INFINITY, l = 0.0f;
         vec o{};
         for (uint32_t i0 = at; i0 < n; i0 += step * kJoinBatch) {
@@ -45,8 +72,8 @@ __global__ __launch_bounds__(kJoinThreads) void rows_attn_join_kernel(AttnRows a
             vec x[kJoinBatch];
 #pragma unroll
             for (int j = 0; j < kJoinBatch; ++j) {
-                const uint32_t i = min(i0 + j * step, n - 1u);
-                const float* rec = base + (2ull * i + (i == 0 ? 1u : 0u)) * size;
+                const uint32_t k = min(i0 + j * step, n - 1u);
+                const float* rec = base + (2ull * k + (k == 0 ? 1u : 0u)) * size;
                 ml[j] = reinterpret_cast<const float2*>(rec + (size_t(DP) << a.row_shift))[r];
                 x[j] = *reinterpret_cast<const vec*>(rec + size_t(r) * DP + lane * PER);
             }
@@ -76,61 +103,101 @@ __global__ __launch_bounds__(kJoinThreads) void rows_attn_join_kernel(AttnRows a
         const uint32_t d = (all ? threadIdx.x : lane) * 4;
         if (d < a.head_dim && p.past + int32_t(t) >= 0) {
             const uint32_t v0 = all ? 0u : wave, v1 = all ? kJoinWaves : wave + 1u;
-            float most = -INFINITY, sum = 0.0f;
+            float most = -INFINITY, s = 0.0f;
             for (uint32_t v = v0; v < v1; ++v) most = fmaxf(most, s_ml[v].x);
             f32x4 y{0.0f, 0.0f, 0.0f, 0.0f};
             for (uint32_t v = v0; v < v1; ++v) {
                 const float2 ml = s_ml[v];
                 if (ml.x == -INFINITY) continue;
                 const float f = exp2_hw(ml.x - most);
-                sum += ml.y * f;
+                s += ml.y * f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) y[j] += s_o[v][d + j] * f;
             }
-            store_row4(a, p.first + t, head, d, y, sum);
+            store_row4(a, p.first + t, head, d, y, s);
         }
     }
 }
 
 // ---- which kernel, and how the work is dealt ----------------------------------------
+enum class AttnKind { few, mid, tile };
 struct AttnPlan {
-    bool     few;
-    uint32_t row_shift, tiles, target;     // the most tiles; target 0: a workgroup for each
-    size_t   part_bytes;
+    AttnKind kind;
+    uint32_t row_shift, tiles, target, least_run;     // tiles: at most; target 0: a workgroup for each
 };
 constexpr uint32_t kCus = 256;
-AttnPlan attn_plan(bool paged, uint32_t n_tokens, uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+// Few rows a sequence go to rows_attn_few.hip (a tile of 16 rows reads its keys once, so
+// up to 32). The others to the kernel that takes least by this estimate, in us: `keys`
+// is what a sequence has, as far as the host knows (of a cache, what its tables hold;
+// half of a prompt's tokens on average), a block 64 keys of 128 dims for 128 rows.
+//   mid    8 for each round of workgroups, and 0.075 a key of a wave (a quarter of the keys)
+//   tile   8, and the longer of the longest tile (1.75 a block, 2.4 where workgroups
+//          share CUs) and all blocks at 0.005
+//   list   24 (256 dims: 36) for the second piece and the join, and all blocks at 0.0055
+// Measured, mid / tile / list: prompts of 2000 in 4 heads over 1 of 256 66 / 125 / 56,
+// with a window of 512 36 / 47 / 48; prompts over 8 kv heads of 128 of 100 tokens 9.9 /
+// 11.6 / 16, of 1000 40 / 35 / 55, of 2000 94 / 64 / 102; chunks of 512 over 1000 34 / 44 /
+// 52, of 100 (four) over 1000 27 / 36 / 40, of 64 over 8000 109 / 185 / 37, of 200 over
+// 30000 371 / 665 / 160.
+AttnPlan attn_plan(bool paged, uint32_t n_tokens, uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, double keys,
+                   bool may_list) {
     AttnPlan p{};
     const uint64_t rows = uint64_t(n_tokens) * (heads / kv_heads);
-    const uint32_t seqs = std::min(n_seq, n_tokens);
-    p.few = paged && rows <= uint64_t(seqs) * 2 * kFewRows;
-    const uint32_t tile = p.few ? kFewRows : kTileRows;
-    p.row_shift = uint32_t(__builtin_ctz(tile));
+    const uint32_t seqs = std::min(n_seq, n_tokens), dp = padded_dim(head_dim);
     // every sequence with rows may leave one tile part filled
-    const uint64_t tiles = (rows / tile + seqs) * kv_heads;
-    p.tiles = uint32_t(std::min<uint64_t>(tiles, 0x7FFFFFFFu));
-    if (tiles < (p.few ? 16 : 4) * kCus) {
-        p.target = padded_dim(head_dim) == 256 ? kCus : 2 * kCus;          // what fits the device at once
-        p.part_bytes = size_t(p.target) * (sizeof(JoinTile) + 2 * part_floats(tile, padded_dim(head_dim)) * sizeof(float));
+    auto tiles = [&](uint32_t tile) { return (rows / tile + seqs) * kv_heads; };
+    const uint32_t slots = dp == 256 ? kCus : 2 * kCus;                    // workgroups that run at once
+    bool list = false;
+    if (paged && rows <= uint64_t(seqs) * 2 * kFewRows) {
+        p.kind = AttnKind::few;
+        list = may_list && tiles(kFewRows) < 16 * kCus;
+    } else {
+        const double dims = dp / 128.0, mean = paged ? keys : keys / 2;
+        const double big = double(tiles(kTileRows)), rounds = std::ceil(double(rows) * kv_heads / kMidRows / slots);
+        const double t_mid = 8 * rounds + std::max(rounds * mean, keys) / 4 * 0.075 * dims;
+        const double t_tile = 8 + std::max(keys / 64 * (big > kCus ? 2.4 : 1.75), big * mean / 64 * 0.005) * dims;
+        const double t_list = (dp == 256 ? 36 : 24) + big * mean / 64 * 0.0055 * dims * (dp == 256 ? 2 : 1);
+        list = may_list && t_list < t_mid && t_list < t_tile;
+        p.kind = list || t_tile <= t_mid ? AttnKind::tile : AttnKind::mid;
+    }
+    const uint32_t tile = p.kind == AttnKind::few ? kFewRows : p.kind == AttnKind::mid ? kMidRows : kTileRows;
+    p.row_shift = uint32_t(__builtin_ctz(tile));
+    p.tiles = uint32_t(std::min<uint64_t>(tiles(tile), 0x7FFFFFFFu));
+    if (list) {
+        p.target = slots;
+        static_assert(2 * kCus <= kMostTarget, "the join's table");
+        p.least_run = p.kind == AttnKind::few ? 0 : 2;
     }
     return p;
 }
+size_t part_bytes(const AttnPlan& p, uint32_t head_dim) {
+    return size_t(p.target) * (sizeof(JoinTile) + 2 * part_floats(1u << p.row_shift, padded_dim(head_dim)) * sizeof(float));
+}
 
-int attention_call(const char* fn, AttnRows a, const AttnPlan& p, int cache, bool paged, void* workspace, hipStream_t st) {
+int attention_call(const char* fn, AttnRows a, bool paged, int cache, void* workspace, size_t bytes, hipStream_t st) {
     const uint32_t dp = padded_dim(a.head_dim);
+    double keys = paged ? double(a.most_keys) : double(a.n_tokens) / a.n_seq;
+    if (a.window) keys = std::min(keys, double(a.window) + double(kTileRows) / (a.heads / a.kv_heads));
+    const AttnPlan p = attn_plan(paged, a.n_tokens, a.n_seq, a.heads, a.kv_heads, a.head_dim, keys, workspace != nullptr);
     set_group(a);
     a.row_shift = p.row_shift;
-    a.block_shift = uint32_t(__builtin_ctz(p.few ? kFewWaves * few_keys(dp, elem_bytes(cache)) : tile_keys_of(dp)));
+    a.block_shift = uint32_t(__builtin_ctz(p.kind == AttnKind::few   ? kFewWaves * few_keys(dp, elem_bytes(cache))
+                                           : p.kind == AttnKind::mid ? kMidKeys
+                                                                     : tile_keys_of(dp)));
     // what the list may hold, and 32-bit places in it
     const uint64_t most = uint64_t(p.tiles) * ((uint64_t(a.most_keys) >> a.block_shift) + 4);
-    a.target = workspace && most < 0x7FFFFFFFull ? p.target : 0u;
+    a.target = most < 0x7FFFFFFFull && part_bytes(p, a.head_dim) <= bytes ? p.target : 0u;
+    a.least_run = p.least_run;
     a.target_shift = a.target ? uint32_t(__builtin_ctz(a.target)) : 0u;
     a.most_blocks = uint32_t(std::min<uint64_t>(most, 0x7FFFFFFFu));
     a.part = static_cast<float*>(workspace);
     const uint32_t grid = a.target ? a.target : p.tiles;
-    XP_CHECK(p.few ? launch_few(a, cache, grid, st) : launch_tile(a, cache, paged, grid, st));
+    if (grid >= 1u << 24) return set_error(XP_E_ARG, "%s: %u tokens of %u heads are over 2^24 tiles of %u rows", fn, a.n_tokens, a.heads, 1u << p.row_shift);
+    XP_CHECK(p.kind == AttnKind::few   ? launch_few(a, cache, grid, st)
+             : p.kind == AttnKind::mid ? launch_mid(a, cache, paged, grid, st)
+                                       : launch_tile(a, cache, paged, grid, st));
     if (a.target == 0) return XP_OK;
-    const dim3 join(kJoinSlices, a.target), block(kJoinThreads);
+    const dim3 join(kJoinGrid), block(kJoinThreads);
     if (dp == 64) hipLaunchKernelGGL((rows_attn_join_kernel<64>), join, block, 0, st, a);
     else if (dp == 128) hipLaunchKernelGGL((rows_attn_join_kernel<128>), join, block, 0, st, a);
     else hipLaunchKernelGGL((rows_attn_join_kernel<256>), join, block, 0, st, a);
@@ -169,8 +236,13 @@ int xp_attention_workspace(uint32_t n_tokens, uint32_t n_seq, uint32_t heads, ui
     XP_REQUIRE(bytes, "bytes is null");
     XP_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%u heads are no multiple of %u kv heads", heads, kv_heads);
     XP_REQUIRE(head_dim > 0 && head_dim % 16 == 0 && head_dim <= 256, "head_dim %u is not a multiple of 16 up to 256", head_dim);
-    *bytes = std::max<size_t>({16, attn_plan(true, n_tokens, n_seq, heads, kv_heads, head_dim).part_bytes,
-                               attn_plan(false, n_tokens, n_seq, heads, kv_heads, head_dim).part_bytes});
+    // whatever the lengths: a list of the tiles that rows and sequences may have
+    AttnPlan p = attn_plan(true, n_tokens, n_seq, heads, kv_heads, head_dim, 0, true);
+    size_t most = part_bytes(p, head_dim);
+    p.target = padded_dim(head_dim) == 256 ? kCus : 2 * kCus;
+    p.row_shift = uint32_t(__builtin_ctz(kTileRows));
+    if (p.kind != AttnKind::few) most = part_bytes(p, head_dim);
+    *bytes = std::max<size_t>(most, 16);
     return XP_OK;
 }
 
@@ -188,8 +260,7 @@ int xp_attention_paged(const xp_rows* out, const xp_rows* q, const xp_paged_kv* 
     a.cu = s->cu, a.kv_len = s->kv_len, a.map = page_map(c, s), a.n_seq = s->n_seq, a.n_tokens = s->n_tokens;
     a.heads = q->heads, a.kv_heads = c->kv_heads, a.head_dim = c->head_dim, a.window = window, a.q_elem = q->elem, a.scale = scale;
     a.most_keys = int32_t(std::min<uint64_t>(uint64_t(s->table) * c->page_size, kMostKeys));
-    return attention_call(__func__, a, attn_plan(true, a.n_tokens, a.n_seq, a.heads, a.kv_heads, a.head_dim), c->elem, true, workspace,
-                          as_stream(stream));
+    return attention_call(__func__, a, true, c->elem, workspace, workspace_bytes, as_stream(stream));
 }
 
 int xp_attention_packed(const xp_rows* out, const xp_rows* q, const xp_rows* k, const xp_rows* v, uint32_t head_dim,
@@ -211,8 +282,7 @@ int xp_attention_packed(const xp_rows* out, const xp_rows* q, const xp_rows* k, 
     a.cu = cu, a.n_seq = n_seq, a.n_tokens = n_tokens;
     a.heads = q->heads, a.kv_heads = k->heads, a.head_dim = head_dim, a.window = window, a.q_elem = q->elem, a.scale = scale;
     a.most_keys = int32_t(std::min<uint32_t>(n_tokens, kMostKeys));
-    return attention_call(__func__, a, attn_plan(false, n_tokens, n_seq, a.heads, a.kv_heads, head_dim), k->elem, false, workspace,
-                          as_stream(stream));
+    return attention_call(__func__, a, false, k->elem, workspace, workspace_bytes, as_stream(stream));
 }
 
 }  // extern "C"

@@ -39,8 +39,7 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) void rows_attn_few_
     __shared__ Stage s1[kFewWaves];
     __shared__ float2 s_ml[kFewWaves][kFewRows];
 
-    const uint32_t lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const uint32_t n16 = lane % 16, g = lane / 16, group = a.heads / a.kv_heads;
+    const uint32_t group = a.heads / a.kv_heads;
     const uint32_t rowbytes = a.head_dim * SZ, pmask = (1u << a.map.page_shift) - 1u;
 
     __shared__ UnitsLds s_units;
@@ -48,6 +47,9 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) void rows_attn_few_
     SeqWork sw{};
     if (LIST) deal.join(a, Piece{}, sw, 0);
     for (Piece it = deal.next(a, &sw); it.live; it = deal.next(a, &sw)) {
+    // (anew for each piece, or what follows from them is kept through all, in too many registers)
+    const uint32_t tid = LIST ? opaque_tid() : threadIdx.x, lane = tid % kWave, wave = uniform(tid / kWave);
+    const uint32_t n16 = lane % 16, g = lane / 16;
     const uint32_t n_rows = sw.n_new * group, first = sw.first;
     const int32_t past = sw.past;
     const uint32_t r0 = it.tile * kFewRows, r1 = min(r0 + kFewRows, n_rows);

@@ -30,16 +30,18 @@ __device__ __forceinline__ SeqWork lane_work(const AttnRows& a, uint32_t b) {
 __device__ __forceinline__ SeqWork work_of_lane(const SeqWork& w, uint32_t l) {
     return {of_lane(w.first, l), of_lane(w.n_new, l), of_lane(w.tiles, l), int32_t(of_lane(uint32_t(w.past), l))};
 }
-// The units (tiles, or with LIST blocks of the list, of all kv heads) of up to 64
-// sequences a lane each, and their sums up to and with each lane's. (The sums of a
+// The tiles, and with LIST the blocks of the list, of all kv heads of up to 64
+// sequences, a lane each, and their sums up to and with each lane's. (The sums of a
 // cu that gives rows many times over may wrap: the callers bound what they find.)
-template <bool LIST>
 struct LaneUnits {
     SeqWork  w;
     uint32_t own, up;
-    __device__ __forceinline__ void read(const AttnRows& a, uint32_t b0) {
+    __device__ __forceinline__ void read(const AttnRows& a, uint32_t b0, bool blocks) {
         w = lane_work(a, b0 + threadIdx.x % kWave);
-        own = (LIST ? head_list(a, w).blocks : w.tiles) * a.kv_heads;
+        sum(a, blocks);
+    }
+    __device__ __forceinline__ void sum(const AttnRows& a, bool blocks) {
+        own = (blocks ? head_list(a, w).blocks : w.tiles) * a.kv_heads;
         up = wave_scan_add(own);
     }
     __device__ __forceinline__ uint32_t all() const { return of_lane(up, kWave - 1); }
@@ -55,31 +57,38 @@ struct Found {
 struct UnitsLds {
     uint32_t v[6][kWave];
 };
-template <bool LIST>
 struct Units {
     UnitsLds& lds;
     uint32_t  total;
-    __device__ __forceinline__ Units(const AttnRows& a, UnitsLds& s) : lds(s), total(0) {
+    bool      blocks;              // units are blocks of the list, not tiles
+    __device__ __forceinline__ Units(const AttnRows& a, UnitsLds& s, bool list) : lds(s), total(0), blocks(list) {
+        LaneUnits u;
+        u.read(a, 0, list);
+        count(a, u);
+        if (list && total < uint64_t(a.least_run) * a.target) {
+            blocks = false;
+            u.sum(a, false);
+            count(a, u);
+        }
         const uint32_t lane = threadIdx.x % kWave;
-        LaneUnits<LIST> u;
-        u.read(a, 0);
         s.v[0][lane] = u.w.n_new, s.v[1][lane] = u.w.tiles, s.v[2][lane] = uint32_t(u.w.past), s.v[3][lane] = u.own, s.v[4][lane] = u.up;
         s.v[5][lane] = u.w.first;
+    }
+    __device__ __forceinline__ void count(const AttnRows& a, const LaneUnits& u) {
         total = u.all();
-        if (a.n_seq > kWave)
-            for (uint32_t b0 = kWave; b0 < a.n_seq; b0 += kWave) {
-                LaneUnits<LIST> v;
-                v.read(a, b0);
-                total += v.all();
-            }
-        if (LIST) total = min(total, a.most_blocks);
+        for (uint32_t b0 = kWave; b0 < a.n_seq; b0 += kWave) {
+            LaneUnits v;
+            v.read(a, b0, blocks);
+            total += v.all();
+        }
+        total = uniform(min(total, a.most_blocks));
     }
     __device__ __forceinline__ Found find(const AttnRows& a, uint32_t i) const {
         const uint32_t lane = threadIdx.x % kWave;
         uint32_t before = 0;
-        LaneUnits<LIST> v{{lds.v[5][lane], lds.v[0][lane], lds.v[1][lane], int32_t(lds.v[2][lane])}, lds.v[3][lane], lds.v[4][lane]};
+        LaneUnits v{{lds.v[5][lane], lds.v[0][lane], lds.v[1][lane], int32_t(lds.v[2][lane])}, lds.v[3][lane], lds.v[4][lane]};
         for (uint32_t b0 = 0; b0 < a.n_seq; b0 += kWave) {
-            if (b0) v.read(a, b0);
+            if (b0) v.read(a, b0, blocks);
             const uint64_t hit = __ballot(i < before + v.up);
             if (hit) {
                 const uint32_t l = uint32_t(__ffsll(static_cast<long long>(hit))) - 1u;
@@ -92,7 +101,7 @@ struct Units {
 };
 // The piece at place `at` of the list (n up to the tile's end; 0: not live, or a
 // gap of `of`).
-__device__ __forceinline__ Piece list_piece(const AttnRows& a, const Units<true>& units, uint32_t at, SeqWork* work) {
+__device__ __forceinline__ Piece list_piece(const AttnRows& a, const Units& units, uint32_t at, SeqWork* work) {
     const Found f = units.find(a, at);
     Piece p{0, 0, 0, 0, 0, 0, false};
     if (!f.live) return p;
@@ -103,6 +112,15 @@ __device__ __forceinline__ Piece list_piece(const AttnRows& a, const Units<true>
     *work = f.w;
     return {f.seq, uniform(p.tile), uniform(h), uniform(p.blk), uniform(p.n), uniform(p.of), p.live};
 }
+// The call's tile i, whole.
+__device__ __forceinline__ Piece whole_tile(const AttnRows& a, const Units& units, uint32_t i, SeqWork* work) {
+    const Found f = units.find(a, i);
+    const uint32_t tile = f.w.tiles - 1u - f.at / a.kv_heads;
+    if (!f.live || tile >= f.w.tiles) return {0, 0, 0, 0, 0, 0, false};
+    *work = f.w;
+    const uint32_t n = tile_blocks(a, f.w, tile).n;
+    return {f.seq, uniform(tile), uniform(f.at % a.kv_heads), 0, uniform(n), uniform(n), true};
+}
 // Workgroup `block` of the grid as one of the list: neighbours in it share keys, so
 // each XCD (which takes every eighth workgroup) gets an eighth of it.
 __device__ __forceinline__ uint32_t list_wg(const AttnRows& a, uint32_t blocks, uint32_t block) {
@@ -112,10 +130,10 @@ __device__ __forceinline__ uint32_t list_wg(const AttnRows& a, uint32_t blocks, 
 // The pieces of this workgroup, one after the other, with the sequence's work.
 template <bool LIST>
 struct Dealer {
-    Units<LIST> units;
-    uint32_t    at, end, wg;       // of the list
-    __device__ __forceinline__ Dealer(const AttnRows& a, UnitsLds& s) : units(a, s), at(0), end(1), wg(blockIdx.x) {
-        if constexpr (LIST) {
+    Units    units;
+    uint32_t at, end, wg;          // places of the list, or tiles
+    __device__ __forceinline__ Dealer(const AttnRows& a, UnitsLds& s) : units(a, s, LIST), at(blockIdx.x), end(units.total), wg(blockIdx.x) {
+        if (LIST && units.blocks) {
             wg = uniform(list_wg(a, units.total, blockIdx.x));
             at = uniform(wg < units.total ? run_first(a, units.total, wg) : 0u);
             end = uniform(wg < units.total ? run_first(a, units.total, wg + 1) : 0u);
@@ -130,8 +148,15 @@ struct Dealer {
     }
     // (not live at the end)
     __device__ __forceinline__ Piece next(const AttnRows& a, SeqWork* work) {
-        if constexpr (LIST) {
-            while (at < end) {
+        if constexpr (!LIST) {
+            Piece p{0, 0, 0, 0, 0, 0, false};
+            if (wg == blockIdx.x) p = whole_tile(a, units, wg, work);
+            wg = ~0u;                                             // one only
+            p.live = p.live && p.n > 0;
+            return p;
+        }
+        while (at < end) {
+            if (units.blocks) {
                 Piece p = list_piece(a, units, at, work);
                 if (!p.live) break;
                 if (p.n) {
@@ -140,15 +165,11 @@ struct Dealer {
                     return p;
                 }
                 at += p.of;
-            }
-        } else if (at < end) {
-            at = end;
-            const Found f = units.find(a, blockIdx.x);
-            const uint32_t tile = f.w.tiles - 1u - f.at / a.kv_heads;
-            if (f.live && tile < f.w.tiles) {
-                *work = f.w;
-                const uint32_t n = tile_blocks(a, f.w, tile).n;
-                return {f.seq, uniform(tile), uniform(f.at % a.kv_heads), 0, uniform(n), uniform(n), n > 0};
+            } else {
+                const Piece p = whole_tile(a, units, at, work);
+                at += a.target;
+                if (!p.live) break;
+                if (p.n) return p;
             }
         }
         return {0, 0, 0, 0, 0, 0, false};
@@ -441,8 +462,10 @@ XP_HD constexpr uint32_t few_keys(uint32_t dp, uint32_t size) {    // of a wave 
 }
 constexpr uint32_t kTileWaves = 4, kTileRows = 32 * kTileWaves;
 XP_HD constexpr uint32_t tile_keys_of(uint32_t dp) { return dp == 256 ? 32u : 64u; }
+constexpr uint32_t kMidWaves = 4, kMidRows = 32, kMidKeys = 32 * kMidWaves;
 // Launchers; `grid` workgroups.
 int launch_few(const AttnRows& a, int cache, uint32_t grid, hipStream_t st);
+int launch_mid(const AttnRows& a, int cache, bool paged, uint32_t grid, hipStream_t st);
 int launch_tile(const AttnRows& a, int cache, bool paged, uint32_t grid, hipStream_t st);
 
 }  // namespace xp

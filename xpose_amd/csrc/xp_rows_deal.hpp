@@ -19,7 +19,7 @@ struct AttnRows {
     // How the work is dealt (below): rows of a tile and keys of a block (powers of
     // two), the workgroups that share the list (0: a tile each) and where their
     // parts go, the most blocks of the list, the positions of the page table
-    uint32_t    row_shift, block_shift, target, target_shift, most_blocks;
+    uint32_t    row_shift, block_shift, target, target_shift, least_run, most_blocks;
     int32_t     most_keys;
     uint32_t    group_mul, group_shift;    // n / (heads / kv_heads) = n group_mul >> group_shift
     float*      part;
@@ -34,8 +34,10 @@ struct AttnRows {
 // tile: the longest first, the kv head changing fastest, so that the tiles of
 // a head meet in one XCD's L2 where kv_heads shares a factor with 8.
 //
-// Otherwise all blocks of the call, tile after tile, are one list that `target`
-// workgroups share in equal runs. A run's first and last tile may be parts; their
+// Otherwise `target` workgroups share the call, by its lengths, which only the
+// kernel knows. Where a workgroup would get fewer than least_run blocks each takes
+// whole tiles, every target-th of that order. Else all blocks, tile after tile, are one
+// list that they share in equal runs. A run's first and last tile may be parts; their
 // sums go to `part`, two records a workgroup, and the join kernel adds them; whole
 // tiles are written at once. In the list, tile v of a head comes after tile
 // tiles - 1 - v: of a causal prompt such a pair has about the same blocks
