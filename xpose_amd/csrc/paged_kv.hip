@@ -5,8 +5,8 @@
 // each (its largest absolute value is found by exchanges among them), kKvAhead
 // rows at a time, so that each lane has that many loads in flight; where the tokens'
 // rows lie in the cache is found meanwhile, a lane a token, and passed through LDS.
-// 32000 rows of 4 heads of 64 in f16, written and read back: 37.2 us a row at a time, KVA
-// so; 4300 of 8 heads of 128 from bf16 to e4m3 and back 26.6, KVB.
+// 32000 rows of 4 heads of 64 in f16, written and read back: 37.2 us a row at a time, 25.3
+// so (5.2 TB/s); 4700 of 8 heads of 128 from bf16 to e4m3 and back 26.6 and 20.3.
 #include <algorithm>
 
 #include "xp_elem.hpp"
@@ -15,7 +15,8 @@ namespace xp {
 namespace {
 
 constexpr uint32_t kKvThreads = 256;
-constexpr uint32_t kKvAhead = 4, kKvTokens = 64, kKvSeqs = 255;
+constexpr uint32_t kKvAhead = 4;           // rows that a lane sends for at once
+constexpr uint32_t kKvTokens = 64, kKvSeqs = 255;
 
 struct KvRows {
     void *         cache[2];       // k, v
@@ -104,39 +105,58 @@ __device__ __forceinline__ float quantise8(const float (&x)[8], uint32_t top, u3
     }
 }
 
+// The largest of a row's lanes' values, in all of them (lanes a power of two, up to 32).
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    return max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, 0xF, 0xF, true)));
+}
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t lanes) {
+    if (lanes >= 2) v = dpp_max<0xB1>(v);      // quad_perm [1,0,3,2]
+    if (lanes >= 4) v = dpp_max<0x4E>(v);      // quad_perm [2,3,0,1]
+    if (lanes >= 8) v = dpp_max<0x141>(v);     // row_half_mirror
+    if (lanes >= 16) v = dpp_max<0x140>(v);    // row_mirror
+    if (lanes >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max(uint32_t(r[0]), uint32_t(r[1]));
+    }
+    return v;
+}
+
 template <int IN, int CACHE>
 __global__ __launch_bounds__(kKvThreads) void paged_kv_write_kernel(KvRows a) {
     __shared__ KvSlots slots;
     const uint32_t per = kKvThreads / a.lanes, sub = threadIdx.x / a.lanes, lane = threadIdx.x % a.lanes;
     const uint32_t t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.n_tokens - t0), n = nt * a.kv_heads * 2;
     const bool live = lane * 8 < a.head_dim;
-    for (uint32_t i0 = 0; i0 < n; i0 += per * kKvAhead) {
-        float x[kKvAhead][8];
-        KvRow r[kKvAhead];
+    constexpr uint32_t AHEAD = kKvAhead;
+    for (uint32_t i0 = 0; i0 < n; i0 += per * AHEAD) {
+        Raw8<IN> raw[AHEAD];
+        KvRow r[AHEAD];
 #pragma unroll
-        for (uint32_t j = 0; j < kKvAhead; ++j) {
+        for (uint32_t j = 0; j < AHEAD; ++j) {
             const uint32_t i = i0 + j * per + sub;
             r[j] = row_of(a, min(i, n - 1u));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[j][e] = 0.0f;
+            raw[j].zero();
             if (i < n && live)
-                load8<IN>(a.rows[r[j].kv], uint64_t(t0 + r[j].token) * a.stride[r[j].kv] + uint64_t(r[j].head) * a.head_dim + lane * 8, x[j]);
+                raw[j].load(a.rows[r[j].kv], uint64_t(t0 + r[j].token) * a.stride[r[j].kv] + uint64_t(r[j].head) * a.head_dim + lane * 8);
         }
         if (i0 == 0) find_slots(a, slots, t0);
 #pragma unroll
-        for (uint32_t j = 0; j < kKvAhead; ++j) {
+        for (uint32_t j = 0; j < AHEAD; ++j) {
+            float x[8];
+            raw[j].floats(x);
             const int64_t base = slots.at[r[j].token], row = base + (int64_t(r[j].head) << a.map.page_shift);
             const bool put = base >= 0 && i0 + j * per + sub < n;
             const uint64_t to = uint64_t(row) * a.head_dim + lane * 8;
             if constexpr (CACHE == XP_ELEM_F16 || CACHE == XP_ELEM_BF16) {
-                if (put && live) store8<CACHE>(a.cache[r[j].kv], to, x[j]);
+                if (put && live) store8<CACHE>(a.cache[r[j].kv], to, x);
             } else {
                 uint32_t top = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[j][e]) & 0x7FFFFFFFu);
-                for (uint32_t o = 1; o < a.lanes; o <<= 1) top = max(top, uint32_t(__shfl_xor(int(top), int(o), kWave)));
+                for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+                top = row_max(top, a.lanes);
                 u32x2 code;
-                const float scale = quantise8<CACHE>(x[j], top, code);
+                const float scale = quantise8<CACHE>(x, top, code);
                 if (put && live) *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.cache[r[j].kv]) + to) = code;
                 if (put && lane == 0) a.scale[r[j].kv][row] = scale;
             }
@@ -151,26 +171,31 @@ __global__ __launch_bounds__(kKvThreads) void paged_kv_read_kernel(KvRows a) {
     const uint32_t t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.n_tokens - t0), n = nt * a.kv_heads * 2;
     find_slots(a, slots, t0);
     if (lane * 8 >= a.head_dim) return;
-    for (uint32_t i0 = 0; i0 < n; i0 += per * kKvAhead) {
-        float x[kKvAhead][8], s[kKvAhead];
-        KvRow r[kKvAhead];
+    constexpr uint32_t AHEAD = kKvAhead;
+    for (uint32_t i0 = 0; i0 < n; i0 += per * AHEAD) {
+        Raw8<CACHE> raw[AHEAD];
+        float s[AHEAD];
+        KvRow r[AHEAD];
 #pragma unroll
-        for (uint32_t j = 0; j < kKvAhead; ++j) {
+        for (uint32_t j = 0; j < AHEAD; ++j) {
             r[j] = row_of(a, min(i0 + j * per + sub, n - 1u));
             const int64_t base = slots.at[r[j].token], row = max(base, int64_t(0)) + (int64_t(r[j].head) << a.map.page_shift);
             s[j] = 1.0f;
+            raw[j].zero();
             if (base >= 0) {
-                load8<CACHE>(a.cache[r[j].kv], uint64_t(row) * a.head_dim + lane * 8, x[j]);
+                raw[j].load(a.cache[r[j].kv], uint64_t(row) * a.head_dim + lane * 8);
                 if constexpr (CACHE == XP_ELEM_I8 || CACHE == XP_ELEM_E4M3) s[j] = a.scale[r[j].kv][row];
             }
         }
 #pragma unroll
-        for (uint32_t j = 0; j < kKvAhead; ++j) {
+        for (uint32_t j = 0; j < AHEAD; ++j) {
             const int64_t base = slots.at[r[j].token];
             if (i0 + j * per + sub >= n || base == kNoSeq) continue;
+            float x[8];
+            raw[j].floats(x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[j][e] = base < 0 ? __uint_as_float(0x7FC00000u) : CACHE == XP_ELEM_I8 || CACHE == XP_ELEM_E4M3 ? x[j][e] * s[j] : x[j][e];
-            store8<OUT>(a.rows[r[j].kv], uint64_t(t0 + r[j].token) * a.stride[r[j].kv] + uint64_t(r[j].head) * a.head_dim + lane * 8, x[j]);
+            for (int e = 0; e < 8; ++e) x[e] = base < 0 ? __uint_as_float(0x7FC00000u) : CACHE == XP_ELEM_I8 || CACHE == XP_ELEM_E4M3 ? x[e] * s[j] : x[e];
+            store8<OUT>(a.rows[r[j].kv], uint64_t(t0 + r[j].token) * a.stride[r[j].kv] + uint64_t(r[j].head) * a.head_dim + lane * 8, x);
         }
     }
 }

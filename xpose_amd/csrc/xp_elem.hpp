@@ -38,27 +38,48 @@ __device__ __forceinline__ void store1(void* base, uint64_t i, float x) {
     else static_cast<uint16_t*>(base)[i] = uint16_t(pack_bf16(x, x));
 }
 
-// Eight elements from the element index i on (32 bytes of f32, 16 of 16 bits,
-// 8 of 8 bits, aligned to that or to 16).
+// Eight elements as they lie in memory: 32 bytes of f32, 16 of 16 bits, 8 of 8 bits,
+// aligned to that or to 16.
 template <int ELEM>
-__device__ __forceinline__ void load8(const void* base, uint64_t i, float (&x)[8]) {
-    if constexpr (ELEM == XP_ELEM_F32) {
+struct Raw8 {
+    u32x4 a, b;
+    __device__ __forceinline__ void load(const void* base, uint64_t i) {
         const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const float*>(base) + i);
-        const u32x4 a = p[0], b = p[1];
+        a = p[0];
+        b = p[1];
+    }
+    __device__ __forceinline__ void zero() { a = b = u32x4{0u, 0u, 0u, 0u}; }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(a[j]), x[4 + j] = __uint_as_float(b[j]);
-    } else if constexpr (ELEM == XP_ELEM_F16 || ELEM == XP_ELEM_BF16) {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + i);
+    }
+};
+template <bool F16>
+struct Raw8x16 {
+    u32x4 a;
+    __device__ __forceinline__ void load(const void* base, uint64_t i) {
+        a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + i);
+    }
+    __device__ __forceinline__ void zero() { a = u32x4{0u, 0u, 0u, 0u}; }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            x[2 * j] = ELEM == XP_ELEM_F16 ? f16_lo(a[j]) : bf16lo(a[j]);
-            x[2 * j + 1] = ELEM == XP_ELEM_F16 ? f16_hi(a[j]) : bf16hi(a[j]);
+            x[2 * j] = F16 ? f16_lo(a[j]) : bf16lo(a[j]);
+            x[2 * j + 1] = F16 ? f16_hi(a[j]) : bf16hi(a[j]);
         }
-    } else {
-        const u32x2 a = *reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(base) + i);
+    }
+};
+template <bool I8>
+struct Raw8x8 {
+    u32x2 a;
+    __device__ __forceinline__ void load(const void* base, uint64_t i) {
+        a = *reinterpret_cast<const u32x2*>(static_cast<const uint8_t*>(base) + i);
+    }
+    __device__ __forceinline__ void zero() { a = u32x2{0u, 0u}; }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-            if constexpr (ELEM == XP_ELEM_I8) {
+            if constexpr (I8) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[4 * w + j] = float(int8_t(a[w] >> (8 * j)));
             } else {
@@ -68,6 +89,17 @@ __device__ __forceinline__ void load8(const void* base, uint64_t i, float (&x)[8
             }
         }
     }
+};
+template <> struct Raw8<XP_ELEM_F16> : Raw8x16<true> {};
+template <> struct Raw8<XP_ELEM_BF16> : Raw8x16<false> {};
+template <> struct Raw8<XP_ELEM_I8> : Raw8x8<true> {};
+template <> struct Raw8<XP_ELEM_E4M3> : Raw8x8<false> {};
+
+template <int ELEM>
+__device__ __forceinline__ void load8(const void* base, uint64_t i, float (&x)[8]) {
+    Raw8<ELEM> r;
+    r.load(base, i);
+    r.floats(x);
 }
 template <int ELEM>
 __device__ __forceinline__ void store8(void* base, uint64_t i, const float (&x)[8]) {
