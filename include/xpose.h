@@ -445,7 +445,8 @@ typedef struct {
 int xp_rope_frequencies(const xp_rope_spec* r, double* f, uint32_t n);
 /* Turns token t of q (and of k, in the same launch; k and k_out may both be
  * NULL) by positions[t], a signed 32-bit position in device memory (a negative
- * one turns back). Angles are exact to 2^-32 of a turn at any position. An
+ * one turns back). Angles are off by at most 2^-24 of a turn at any position
+ * (2^-31 up to 2^20 or so), and cosines and sines by two roundings. An
  * output may be its input (turned in place) or not overlap it; it has its
  * input's heads and elem. head_dim is even and at most 512; here data and
  * stride need only the element's own alignment (fastest where both are
