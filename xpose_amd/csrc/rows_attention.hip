@@ -5,9 +5,10 @@
 // sum make it one pass over the keys: when the maximum rises from m to m', what
 // has been summed is multiplied by exp(m - m').
 //
-// The products are made by two kernels, for few rows a sequence
-// (rows_attn_few.hip) and for many (rows_attn_tile.hip). Where the rows alone
-// leave CUs without work the keys are split, and a second kernel joins the parts.
+// The products are made by three kernels: for few rows a sequence (rows_attn_few.hip,
+// tiles of 16), for many (rows_attn_tile.hip, 128), and for prompts whose tiles of 128
+// would leave CUs without work (rows_attn_mid.hip, 32). The first two may also take the
+// blocks of all tiles as one list in equal runs, whose parts the kernel below joins.
 #include <algorithm>
 #include <cmath>
 
@@ -126,33 +127,45 @@ struct AttnPlan {
     uint32_t row_shift, tiles, target, least_run;     // tiles: at most; target 0: a workgroup for each
 };
 constexpr uint32_t kCus = 256;
-// Few rows a sequence go to rows_attn_few.hip (a tile of 16 rows reads its keys once, so
-// up to 32). The others to the kernel that takes least by this estimate, in us: `keys`
+// Few rows a sequence of a cache go to rows_attn_few.hip (a tile of 16 rows reads its keys
+// once, so up to 32), the others to the kernel that takes least by this estimate, in us: `keys`
 // is what a sequence has, as far as the host knows (of a cache, what its tables hold;
 // half of a prompt's tokens on average), a block 64 keys of 128 dims for 128 rows.
 //   mid    8 for each round of workgroups, and 0.075 a key of a wave (a quarter of the keys)
 //   tile   8, and the longer of the longest tile (1.75 a block, 2.4 where workgroups
 //          share CUs) and all blocks at 0.005
 //   list   24 (256 dims: 36) for the second piece and the join, and all blocks at 0.0055
+// and of the first kernel, with all it reads, tables taken as half full, at 7 bytes a ps:
+//   tiles  4.5 (7), and 0.0095 a key of 128 dims in the longest, or all, and half that
+//   list   12 (13.5) with the join, 11 a tile that a workgroup takes, and all
 // Measured, mid / tile / list: prompts of 2000 in 4 heads over 1 of 256 66 / 125 / 56,
 // with a window of 512 36 / 47 / 48; prompts over 8 kv heads of 128 of 100 tokens 9.9 /
 // 11.6 / 16, of 1000 40 / 35 / 55, of 2000 94 / 64 / 102; chunks of 512 over 1000 34 / 44 /
 // 52, of 100 (four) over 1000 27 / 36 / 40, of 64 over 8000 109 / 185 / 37, of 200 over
 // 30000 371 / 665 / 160.
-AttnPlan attn_plan(bool paged, uint32_t n_tokens, uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, double keys,
-                   bool may_list) {
+// Of the first, single rows over 8 kv heads of 128, tiles / list: 1 sequence of 100 4.5 / 8.7,
+// of 500 8.5 / 11.0, of 1000 13.8 / 11.1, of 2000 23 / 11; 16 of 500 10.5 / 16, of 2000 27 /
+// 29; 64 up to 2000 55 / 63, up to 8000 197 / 179; 256 up to 2000 179 / 215; 4 heads over 1 of
+// 256, F32 over F16, 1 of 130 10.1 / 13.4, of 400 15.5 / 13.8, of 2000 48 / 14.
+bool few_rows(uint64_t rows, uint32_t seqs) { return rows <= uint64_t(seqs) * 2 * kFewRows; }
+uint32_t slots_of(uint32_t dp) { return dp == 256 ? kCus : 2 * kCus; }      // workgroups that run at once
+AttnPlan attn_plan(bool paged, uint32_t n_tokens, uint32_t n_seq, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t bytes,
+                   double keys, bool may_list) {
     AttnPlan p{};
     const uint64_t rows = uint64_t(n_tokens) * (heads / kv_heads);
     const uint32_t seqs = std::min(n_seq, n_tokens), dp = padded_dim(head_dim);
     // every sequence with rows may leave one tile part filled
     auto tiles = [&](uint32_t tile) { return (rows / tile + seqs) * kv_heads; };
-    const uint32_t slots = dp == 256 ? kCus : 2 * kCus;                    // workgroups that run at once
+    const uint32_t slots = slots_of(dp);
     bool list = false;
-    if (paged && rows <= uint64_t(seqs) * 2 * kFewRows) {
+    const double dims = dp / 128.0;
+    if (paged && few_rows(rows, seqs)) {
         p.kind = AttnKind::few;
-        list = may_list && tiles(kFewRows) < 16 * kCus;
+        const double n = double(tiles(kFewRows)), all = n * keys / 2 * (2.0 * dp * bytes) / 7e6, longest = 0.0095 * dims * keys;
+        const double t_tiles = (dp == 256 ? 7 : 4.5) + std::max(longest, all + longest / 2);
+        list = may_list && (dp == 256 ? 13.5 : 12) + 11 * n / slots + all < t_tiles;
     } else {
-        const double dims = dp / 128.0, mean = paged ? keys : keys / 2;
+        const double mean = paged ? keys : keys / 2;
         const double big = double(tiles(kTileRows)), rounds = std::ceil(double(rows) * kv_heads / kMidRows / slots);
         const double t_mid = 8 * rounds + std::max(rounds * mean, keys) / 4 * 0.075 * dims;
         const double t_tile = 8 + std::max(keys / 64 * (big > kCus ? 2.4 : 1.75), big * mean / 64 * 0.005) * dims;
@@ -170,15 +183,15 @@ AttnPlan attn_plan(bool paged, uint32_t n_tokens, uint32_t n_seq, uint32_t heads
     }
     return p;
 }
-size_t part_bytes(const AttnPlan& p, uint32_t head_dim) {
-    return size_t(p.target) * (sizeof(JoinTile) + 2 * part_floats(1u << p.row_shift, padded_dim(head_dim)) * sizeof(float));
+size_t part_bytes(uint32_t target, uint32_t tile, uint32_t head_dim) {
+    return size_t(target) * (sizeof(JoinTile) + 2 * part_floats(tile, padded_dim(head_dim)) * sizeof(float));
 }
 
 int attention_call(const char* fn, AttnRows a, bool paged, int cache, void* workspace, size_t bytes, hipStream_t st) {
     const uint32_t dp = padded_dim(a.head_dim);
     double keys = paged ? double(a.most_keys) : double(a.n_tokens) / a.n_seq;
     if (a.window) keys = std::min(keys, double(a.window) + double(kTileRows) / (a.heads / a.kv_heads));
-    const AttnPlan p = attn_plan(paged, a.n_tokens, a.n_seq, a.heads, a.kv_heads, a.head_dim, keys, workspace != nullptr);
+    const AttnPlan p = attn_plan(paged, a.n_tokens, a.n_seq, a.heads, a.kv_heads, a.head_dim, elem_bytes(cache), keys, workspace != nullptr);
     set_group(a);
     a.row_shift = p.row_shift;
     a.block_shift = uint32_t(__builtin_ctz(p.kind == AttnKind::few   ? kFewWaves * few_keys(dp, elem_bytes(cache))
@@ -186,7 +199,7 @@ int attention_call(const char* fn, AttnRows a, bool paged, int cache, void* work
                                                                      : tile_keys_of(dp)));
     // what the list may hold, and 32-bit places in it
     const uint64_t most = uint64_t(p.tiles) * ((uint64_t(a.most_keys) >> a.block_shift) + 4);
-    a.target = most < 0x7FFFFFFFull && part_bytes(p, a.head_dim) <= bytes ? p.target : 0u;
+    a.target = most < 0x7FFFFFFFull && part_bytes(p.target, 1u << p.row_shift, a.head_dim) <= bytes ? p.target : 0u;
     a.least_run = p.least_run;
     a.target_shift = a.target ? uint32_t(__builtin_ctz(a.target)) : 0u;
     a.most_blocks = uint32_t(std::min<uint64_t>(most, 0x7FFFFFFFu));
@@ -236,13 +249,9 @@ int xp_attention_workspace(uint32_t n_tokens, uint32_t n_seq, uint32_t heads, ui
     XP_REQUIRE(bytes, "bytes is null");
     XP_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%u heads are no multiple of %u kv heads", heads, kv_heads);
     XP_REQUIRE(head_dim > 0 && head_dim % 16 == 0 && head_dim <= 256, "head_dim %u is not a multiple of 16 up to 256", head_dim);
-    // whatever the lengths: a list of the tiles that rows and sequences may have
-    AttnPlan p = attn_plan(true, n_tokens, n_seq, heads, kv_heads, head_dim, 0, true);
-    size_t most = part_bytes(p, head_dim);
-    p.target = padded_dim(head_dim) == 256 ? kCus : 2 * kCus;
-    p.row_shift = uint32_t(__builtin_ctz(kTileRows));
-    if (p.kind != AttnKind::few) most = part_bytes(p, head_dim);
-    *bytes = std::max<size_t>(most, 16);
+    // whatever the lengths: what a list of the tiles of so many rows takes
+    const bool few = few_rows(uint64_t(n_tokens) * (heads / kv_heads), std::min(n_seq, n_tokens));
+    *bytes = part_bytes(slots_of(padded_dim(head_dim)), few ? kFewRows : kTileRows, head_dim);
     return XP_OK;
 }
 
