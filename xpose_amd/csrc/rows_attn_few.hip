@@ -139,18 +139,17 @@ __global__ __launch_bounds__(kFewThreads, DP == 256 ? 1 : 2) void rows_attn_few_
         for (int x = 0; x < KG; ++x) {
             f32x4 c{0.0f, 0.0f, 0.0f, 0.0f};
             const unsigned char* kr = s.k + (16 * x + n16) * RB;
-            const uint32_t f = NC >= 8 ? fk : swizzle_k<NC>(16 * x + n16);
             if constexpr (SZ == 2) {
 #pragma unroll
                 for (int st = 0; st < QS; ++st) {
-                    const u32x4 kf = *reinterpret_cast<const u32x4*>(kr + 16 * ((4 * st + g) ^ f));
+                    const u32x4 kf = *reinterpret_cast<const u32x4*>(kr + 16 * ((4 * st + g) ^ fk));
                     if constexpr (TERMS == 2) c = mfma16<BF16>(kf, q.lo[st], c);
                     c = mfma16<BF16>(kf, q.hi[st], c);
                 }
             } else {
 #pragma unroll
                 for (int st = 0; st < QS; st += 2) {
-                    const u32x4 kb = *reinterpret_cast<const u32x4*>(kr + 16 * ((2 * st + g) ^ f));
+                    const u32x4 kb = *reinterpret_cast<const u32x4*>(kr + 16 * ((2 * st + g) ^ fk));
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         const u32x2 k0 = widen4<CACHE>(kb[2 * y]), k1 = widen4<CACHE>(kb[2 * y + 1]);

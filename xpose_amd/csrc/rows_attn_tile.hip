@@ -14,7 +14,6 @@ struct KeyTile {
     static constexpr int SZ = R::SZ, RB = R::RB, NC = R::NC, RPI = R::RPI;
     static constexpr int KT = tile_keys_of(DP), LOADS = KT / RPI / int(kTileWaves);   // of a wave
     static_assert(LOADS >= 1 && LOADS * RPI * int(kTileWaves) == KT, "every wave loads whole rows");
-    static_assert(int(kTileWaves) * RPI >= (SZ == 1 ? 16 : 8), "a wave's loads lie alike in their rows' swizzles");
     struct __attribute__((aligned(16))) Stage {
         unsigned char k[KT * RB], v[KT * RB];
         float scale[SZ == 1 ? 2 * KT : 4];
@@ -72,7 +71,8 @@ __global__ __launch_bounds__(kTileThreads, DP == 256 || TERMS == 2 ? 1 : 2) void
         no_row = __ballot(pages < 0);
     };
     // A load takes RPI rows; this lane's 16 bytes of them, the same for all loads of a
-    // wave (they are 4 RPI >= 8 rows apart, and the swizzles of a tile's rows repeat so)
+    // wave (they are 4 RPI rows apart, in which the swizzles repeat)
+    static_assert(swizzle_k<NC>(kTileWaves * RPI) == 0 && swizzle_v<NC, SZ == 1, 3>(kTileWaves * RPI) == 0);
     const uint64_t kst = PAGED ? rowbytes : a.k_stride * SZ, vst = PAGED ? rowbytes : a.v_stride * SZ;
     const uint32_t rt0 = wave * RPI + lane / NC;
     const uint32_t ck = 16u * ((lane % NC) ^ swizzle_k<NC>(rt0)), cv = 16u * ((lane % NC) ^ swizzle_v<NC, SZ == 1, 3>(rt0));

@@ -252,23 +252,25 @@ __device__ __forceinline__ u32x2 widen4(uint32_t w) {
 }
 
 // ---- tiles in LDS -------------------------------------------------------------------
-// A tile holds keys as rows of DP elements in 16-byte chunks. A row is a
-// multiple of 64 or 128 bytes, so the chunks of eight keys that a wave reads at
-// once would meet in the same banks: chunk c of a key lies in place c ^ f(key).
-// K is read a chunk a lane, eight following keys at a time. V is read
-// transposed: 16 lanes take 4 keys of 32 bytes (16-bit elements) or 8 keys of 16
-// bytes (8-bit ones: keys 4 h + 0..3 and, 8 or 16 on, four more), so there f takes other bits.
+// A tile holds keys as rows of DP elements in 16-byte chunks; chunk c of a key lies in
+// place c ^ f(key), so that what a wave reads at once meets each of the 64 banks once: a
+// line of 256 bytes, which holds up to four short rows. Of K a lane reads a chunk, 16
+// following keys at a time (as f has it 6.7 cycles a read, with eight values of f for 16
+// keys 8.3; rows of 32 chunks all the same get eight, as sixteen take more registers
+// than there are: a prompt of 8192, 16 heads over 4 of 256, 892 us so, 988 with sixteen). V is read transposed, half a wave at a time: 16-bit elements as four
+// following keys of 64 bytes in the kernels of 32 rows (HI 3), eight of 32 in that of 16
+// (HI 4); 8-bit ones as keys 0..3 and 8..11 of 32 bytes, and keys 0..7 and 16..23 of 16.
 template <int CHUNKS>
-__device__ __forceinline__ uint32_t swizzle_k(uint32_t key) {
-    if constexpr (CHUNKS >= 8) return ((key & 3u) << 1) | ((key >> 2) & 1u);
-    else return (key >> 1) & 3u;
+__device__ __forceinline__ constexpr uint32_t swizzle_k(uint32_t key) {
+    return CHUNKS >= 32 ? ((key & 3u) << 1) | ((key >> 2) & 1u) : CHUNKS == 16 ? key & 15u : CHUNKS == 8 ? (key >> 1) & 7u : (key >> 2) & 3u;
 }
-// (HI: the bit that tells the second four of such eight keys from the first)
 template <int CHUNKS, bool BYTES, int HI>
-__device__ __forceinline__ uint32_t swizzle_v(uint32_t key) {
-    if constexpr (!BYTES) return swizzle_k<CHUNKS>(key);
-    else if constexpr (CHUNKS >= 8) return ((key & 3u) << 1) | ((key >> HI) & 1u);
-    else return ((key >> 1) & 1u) | ((key >> (HI - 1)) & 2u);
+__device__ __forceinline__ constexpr uint32_t swizzle_v(uint32_t key) {
+    constexpr int LINE = CHUNKS >= 16 ? 0 : CHUNKS == 8 ? 1 : 2;         // log2 of the rows in 256 bytes
+    if constexpr (!BYTES) return HI == 3 ? ((key & 3u) >> LINE) << 2 : ((key & 7u) >> LINE) << 1;
+    const uint32_t far = (key >> HI) & 1u;
+    if constexpr (HI == 3) return (((key & 3u) >> LINE) | (far << (2 - LINE))) << 1;
+    else return ((key & 7u) >> LINE) | (far << (3 - LINE));
 }
 
 // Loads straight into LDS, lane l's 16 (4) bytes to lds + 16 l (4 l): from a
