@@ -337,3 +337,152 @@ def test_gpu_a_server_step(xp, cache, elem, page):
             if scale is not None:
                 c.c.scale[w][int(c.s.table[b, p // page]), :, p % page] = scale
     c.check(out.host())
+
+
+def wide_table(new, past, page, positions=8192, seed=5):
+    """(page table of `positions` positions a sequence, pages): the pages in use in any order, none behind them."""
+    used = [-(-(n + p) // page) for n, p in zip(new, past)]
+    order = torch.randperm(sum(used) + 1, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+    table = torch.full((len(new), positions // page), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(used):
+        table[b, :n] = order[at:at + n]
+        at += n
+    return table, sum(used) + 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,past,heads,kvh,dim,elem,cache,page,window", PAGED)
+def test_gpu_attention_paged_in_wide_tables(xp, new, past, heads, kvh, dim, elem, cache, page, window):
+    """Tables with room for 8192 positions, as a server's are: the host takes the call for a long one."""
+    table, pages = wide_table(new, past, page)
+    c = Paged(xp, new, past, heads, kvh, dim, elem, cache, page, window, n_pages=pages, table=table)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("new,past", [([1, 1, 1], [100, 20, 60]), ([70, 3, 90], [100, 30, 0])])
+@pytest.mark.parametrize("cache,elem", [("f16", "f16"), ("i8", "bf16"), ("bf16", "bf16"), ("e4m3", "f32")])
+def test_gpu_attention_paged_wide_tables_with_bad_pages(xp, cache, elem, new, past, window):
+    table, pages = wide_table(new, past, 16)
+    table[0, 3], table[2, 4] = -1, pages
+    c = Paged(xp, new, past, 4, 2, 64, elem, cache, 16, window, n_pages=pages, table=table)
+    if cache in ("f16", "bf16"):                          # and values that are not finite
+        c.c.code[1][int(table[1, 0]), :, 3, 7] = math.inf
+        c.c.code[0][int(table[1, 1]), :, 2, 1] = math.nan
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [True, False])
+@pytest.mark.parametrize("elem,cache,positions", [("bf16", "i8", 512), ("f16", "f16", 8192), ("f32", "e4m3", 8192)])
+def test_gpu_attention_paged_many_sequences(xp, elem, cache, positions, split):
+    """More sequences than a wave has lanes several times over, some with no row, a few of a chunk; two share their pages."""
+    n = 300
+    new = [0 if i % 7 == 3 else 9 if i % 50 == 1 else 1 for i in range(n)]
+    past = [(i * 37) % 250 for i in range(n)]
+    table, pages = wide_table(new, past, 16, positions)
+    new[20] = new[21] = 1
+    past[20] = past[21] = 40
+    table[21, :3] = table[20, :3] = torch.arange(3)
+    c = Paged(xp, new, past, 4, 2, 32, elem, cache, 16, n_pages=pages, table=table, split=split)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [1, 1 << 30, (1 << 32) - 1])
+@pytest.mark.parametrize("new,past", [([1, 1], [600, 0]), ([70, 20], [50, 300])])
+def test_gpu_attention_paged_least_and_largest_windows(xp, new, past, window):
+    for positions in (1024, 8192):
+        table, pages = wide_table(new, past, 16, positions)
+        c = Paged(xp, new, past, 4, 2, 64, "f16", "f16", 16, window, n_pages=pages, table=table)
+        c.check(c.run())
+
+
+@pytest.mark.gpu
+def test_gpu_attention_calls_on_two_streams(xp):
+    """Two calls at once, a workspace each, and the one of the other's sizes after it in the same stream."""
+    calls = []
+    for i, (new, past, elem, cache) in enumerate((([1, 1, 1], [4000, 300, 1999], "bf16", "i8"), ([40, 1, 100], [500, 3000, 0], "f16", "f16"))):
+        table, pages = wide_table(new, past, 16)
+        c = Paged(xp, new, past, 8, 2, 128, elem, cache, 16, n_pages=pages, table=table, seed=i + 1)
+        calls.append((c, c.run()))
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for c, _ in calls:
+        c.dout.buf.upload(U.raw(torch.full_like(c.q, 5.0)))
+    for _ in range(20):
+        for (c, _), st in zip(calls, streams):
+            xp.call("xp_attention_paged", *c.args, st.cuda_stream)
+    torch.cuda.synchronize()
+    for c, alone in calls:
+        assert torch.equal(c.dout.host().view(torch.int16), alone.view(torch.int16))
+        c.check(alone)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("elem,cache", [("f16", "f16"), ("bf16", "i8")])
+@pytest.mark.parametrize("cu", [[0, 9, 4, 20], [-5, 30, 30, 2], [7, 3, 50, 1 << 30]])
+def test_gpu_malformed_sequences_keep_to_their_rows(xp, elem, cache, cu):
+    """A cu that falls or leaves the rows: whatever the call makes of it, nothing outside the descriptors changes."""
+    heads, kvh, dim, page, n = 4, 2, 64, 16, 12
+    for positions in (64, 8192):
+        table, pages = wide_table([9, 9, 9], [20, 3, 30], page, positions)
+        c = Paged(xp, [4, 4, 4], [20, 3, 30], heads, kvh, dim, elem, cache, page, n_pages=pages, table=table, pad=0)
+        c.s.dev[0].buf.upload(np.array(cu, np.int32))
+        c.c.upload()
+        guard = torch.full((3 * n, heads, dim), 5.0).to(DT[elem])
+        dq, dout = Dev(xp, torch.randn(3 * n, heads, dim).to(DT[elem])), Dev(xp, guard)
+        at = lambda d, h: U.rows(xp, d, h, elem, heads * dim, n * heads * dim)  # noqa: E731
+        ws = workspace(xp, n, 3, heads, kvh, dim, True)
+        xp.call("xp_attention_paged", at(dout, heads), at(dq, heads), c.c.desc, c.s.desc, 0, 0.1, *ws, None)
+        xp.call("xp_attention_packed", at(dout, heads), at(dq, heads), at(dq, kvh), at(dq, kvh), dim, 3, n, c.s.dev[0].ptr, 0, 0.1, *ws, None)
+        xp.call("xp_paged_kv_write", c.c.desc, c.s.desc, at(dq, kvh), at(dq, kvh), None)
+        xp.call("xp_paged_kv_read", c.c.desc, c.s.desc, at(dout, kvh), at(dout, kvh), None)
+        xp.synchronize()
+        got = dout.host()
+        assert (got[:n] == 5.0).all() and (got[2 * n:] == 5.0).all()
+
+
+def few_of_packed(xp, qkv, got, heads, kvh, dim, elem, window, every):
+    """Every `every`-th query of one prompt against float64."""
+    x = qkv.to(F64)
+    n = x.shape[0]
+    for i in sorted(set(range(0, n, every)) | {n - 1}):
+        want, size, most = U.attend(x[i:i + 1, :heads], x[:i + 1, heads:heads + kvh], x[:i + 1, heads + kvh:], dim ** -0.5, window, i)
+        # (over 4096 keys the bound's sums have up to twice the roundings, 2^-14 for 2^-15)
+        bound = U.attention_bound(want, size, most, elem, elem) + 2.0 ** -15 * size
+        assert ((got[i:i + 1].to(F64) - want).abs() <= bound).all(), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,heads,kvh,dim,elem,window", [(5000, 2, 1, 256, "f16", 0), (6001, 3, 1, 128, "bf16", 0), (7000, 4, 1, 64, "f16", 3000),
+                                                         (5000, 2, 2, 96, "bf16", 4500)])
+def test_gpu_attention_packed_long_prompts_and_graph(xp, n, heads, kvh, dim, elem, window):
+    """One long prompt of few heads, whose keys are split; captured, and replayed on another prompt and a shorter one."""
+    g = torch.Generator().manual_seed(n)
+    row = (heads + 2 * kvh) * dim
+    cu = torch.tensor([0, n], dtype=torch.int32)
+    d, dcu = Dev(xp, torch.zeros(n, heads + 2 * kvh, dim).to(DT[elem])), Dev(xp, cu)
+    out = Dev(xp, torch.zeros(n, heads, dim).to(DT[elem]))
+    view = lambda h, o: U.rows(xp, d, h, elem, row, o * dim)  # noqa: E731
+    call = (U.rows(xp, out, heads, elem, heads * dim), view(heads, 0), view(kvh, heads), view(kvh, heads + kvh), dim, 1, n, dcu.ptr, window,
+            dim ** -0.5, *workspace(xp, n, 1, heads, kvh, dim, True))
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        xp.call("xp_attention_packed", *call, side.cuda_stream)
+    for length in (n, n, 700):
+        qkv = (torch.randn(n, heads + 2 * kvh, dim, generator=g) * 1.3).to(DT[elem])
+        d.buf.upload(U.raw(qkv))
+        dcu.buf.upload(np.array([0, length], np.int32))
+        out.buf.upload(U.raw(torch.full((n, heads, dim), 5.0).to(DT[elem])))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.host()
+        assert (got[length:] == 5.0).all()
+        few_of_packed(xp, qkv[:length], got, heads, kvh, dim, elem, window, max(1, length // 40))
+        xp.call("xp_attention_packed", *call, None)       # the same without a graph
+        xp.synchronize()
+        assert torch.equal(out.host().view(torch.int16), got.view(torch.int16))

@@ -399,3 +399,35 @@ def test_gpu_outputs_have_to_be_device_memory(xp):
         xp.call("xp_rope_rows", r(at), r(dev.ptr), None, None, pos.ptr, 1, 64, rope_spec(xp), None)
     xp.call("xp_rope_rows", r(dev.ptr), r(dev.ptr), None, None, pos.ptr, 1, 64, rope_spec(xp), None)   # and no error is left behind
     xp.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache,elem", [("i8", "f32"), ("bf16", "f16")])
+def test_gpu_paged_kv_many_sequences(xp, cache, elem):
+    """Hundreds of sequences, many without a new row: what is written is what is read, and nothing else is."""
+    g = torch.Generator().manual_seed(12)
+    n, page, kvh, dim = 700, 16, 2, 32
+    new = [(0, 1, 1, 5, 0, 2, 17)[i % 7] for i in range(n)]
+    lens = [x + (i * 13) % 30 for i, x in enumerate(new)]
+    pages = n * 3 + 1
+    c = U.Cache(xp, g, cache, pages, page, kvh, dim).upload()
+    s = U.Seqs(xp, new, lens, page, pages, n_tokens=sum(new) + 2, g=g, width=3)
+    kv = torch.randn(s.n_tokens, 2 * kvh, dim, generator=g).to(DT[elem])
+    d, back = Dev(xp, kv), Dev(xp, torch.full_like(kv, 5.0))
+    view = lambda t, w: U.rows(xp, t, kvh, elem, 2 * kvh * dim, w * kvh * dim)  # noqa: E731
+    xp.call("xp_paged_kv_write", c.desc, s.desc, view(d, 0), view(d, 1), None)
+    xp.call("xp_paged_kv_read", c.desc, s.desc, view(back, 0), view(back, 1), None)
+    xp.synchronize()
+    got = back.host()
+    assert (got[sum(new):] == 5.0).all()
+    code, scale = U.quantise(kv[:sum(new)], cache)
+    x = code.to(torch.float32)
+    x = (x if scale is None else x * scale[..., None]).to(DT[elem])
+    assert torch.equal(got[:sum(new)], x)
+    # the slots that no token has are as they were
+    want = [t.clone() for t in c.code]
+    for t, b, p in s.tokens():
+        for w in (0, 1):
+            want[w][int(s.table[b, p // page]), :, p % page] = code[t, w * kvh:(w + 1) * kvh]
+    for w in (0, 1):
+        assert torch.equal(c.dcode[w].host().view(torch.uint8), want[w].view(torch.uint8))
