@@ -469,18 +469,20 @@ int xp_paged_kv_read(const xp_paged_kv* c, const xp_paged_seqs* s, const xp_rows
  * cache, which holds their own rows too: the query at position p sees the
  * positions (p - window, p] (all up to p when window is 0),
  *   out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j,   scale > 0,
- * kv head h / (heads / kv_heads). A sequence has at most 2^30 positions. A query that sees a position without a row
+ * kv head h / (heads / kv_heads). A sequence has at most 2^30 positions (a
+ * longer kv_len is taken as that). A query that sees a position without a row
  * in the cache gets NaN; what it does not see, not finite or not, does not
  * reach it. Queries of any elem over F16, I8 and E4M3, of BF16 over BF16; F16
  * queries are taken as they are, BF16 and F32 ones over a cache of another
  * type as powers of two times F16 terms (F32: two terms). out has q's heads
- * and elem and must not overlap q.
+ * and elem and must not overlap q or the cache. More than
+ * 2^24 tiles of 16 to 128 rows are refused.
  *
- * workspace: where there are too few rows for the device's CUs the keys are
- * split, and the parts meet in workspace_bytes (at least what
- * xp_attention_workspace gives, 16-byte aligned). It is written before it is
- * read in every call, and calls that may run at once need one each. NULL: the
- * keys are not split. */
+ * workspace: where there are too few rows for the device's CUs, or lengths too
+ * different, the keys are split, and the parts meet in workspace_bytes (at
+ * least what xp_attention_workspace gives, 16-byte aligned; 4 to 9 MB for single
+ * tokens, 35 to 68 MB for more). It is written before it is read in every call,
+ * and calls that may run at once need one each. NULL: the keys are not split. */
 int xp_attention_paged(const xp_rows* out, const xp_rows* q, const xp_paged_kv* c, const xp_paged_seqs* s,
                        uint32_t window, float scale, void* workspace, size_t workspace_bytes,
                        xp_stream stream);
@@ -492,7 +494,8 @@ int xp_attention_packed(const xp_rows* out, const xp_rows* q, const xp_rows* k, 
                         uint32_t window, float scale, void* workspace, size_t workspace_bytes,
                         xp_stream stream);
 /* Bytes that suffice for any call of these sizes, whatever its lengths (host
- * only). */
+ * only); with n_seq 1, for any call of up to n_tokens tokens and any number of
+ * sequences. */
 int xp_attention_workspace(uint32_t n_tokens, uint32_t n_seq, uint32_t heads, uint32_t kv_heads,
                            uint32_t head_dim, size_t* bytes);
 

@@ -486,3 +486,13 @@ def test_gpu_attention_packed_long_prompts_and_graph(xp, n, heads, kvh, dim, ele
         xp.call("xp_attention_packed", *call, None)       # the same without a graph
         xp.synchronize()
         assert torch.equal(out.host().view(torch.int16), got.view(torch.int16))
+
+
+@pytest.mark.parametrize("dim", [16, 64, 128, 256])
+@pytest.mark.parametrize("heads,kvh", [(1, 1), (32, 8), (40, 1)])
+def test_workspace_of_one_sequence_suffices_for_any_number(xh, heads, kvh, dim):
+    sizes = (1, 2, 7, 8, 9, 31, 32, 33, 64, 1000, 5000)
+    for most in sizes:
+        need = xh.attention_workspace(most, 1, heads, kvh, dim)
+        for n in (x for x in sizes if x <= most):
+            assert all(xh.attention_workspace(n, b, heads, kvh, dim) <= need for b in (1, 2, 5, 64, 4000))

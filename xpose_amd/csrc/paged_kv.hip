@@ -6,7 +6,8 @@
 // rows at a time, so that each lane has that many loads in flight; where the tokens'
 // rows lie in the cache is found meanwhile, a lane a token, and passed through LDS.
 // 32000 rows of 4 heads of 64 in f16, written and read back: 37.2 us a row at a time, 25.3
-// so (5.2 TB/s); 4700 of 8 heads of 128 from bf16 to e4m3 and back 26.6 and 20.3.
+// to 27.6
+// so (a copy reaches 26.7); 4700 of 8 heads of 128 from bf16 to e4m3 and back 26.6 and 19.1.
 #include <algorithm>
 
 #include "xp_elem.hpp"

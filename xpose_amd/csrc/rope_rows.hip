@@ -6,6 +6,10 @@
 // fraction's own 2^-55 at most (in fp32 the product alone is off by a thousandth of a
 // turn at position 10^5). Its high word, signed, is the
 // fraction of a turn in [-1/2, 1/2) that sincospif takes.
+//
+// Bytes bound it. A workgroup's few tokens share their cosines and sines, and a lane takes
+// 16 bytes at a time: 8192 tokens of 40 heads of 128 in bf16 (168 MB) 35.3 us, 4.75 TB/s, what a
+// copy reaches. 16 tokens take 3.1 us of the device and 5.0 of the host.
 #include <algorithm>
 #include <cmath>
 

@@ -6,7 +6,11 @@
 // takes the weights. Nothing passes between lanes but a row's maximum.
 //
 // Bytes bound it: a wave sends its next 8 to 16 KB of K and V straight to LDS of its
-// own while it works on the last, without a barrier until the waves' sums meet.
+// own while it works on the last, without a barrier until the waves' sums meet. 64 single
+// tokens over up to 8000 positions (8 kv heads of 128 in bf16, 1.1 GB) take 180 us, 6.2 TB/s (a
+// wave that only loads reaches 7.0), 16 over 32768 in 8 bits (1.1 GB) 182 us; as tiles alone,
+// without the list, 194 and 329. One over 4096 positions of one head of 256 takes 15 us (86):
+// launch, four dependent reads (lengths, pages, keys, and once more in the join), 4 MB.
 #include "xp_rows_attn.hpp"
 
 namespace xp {

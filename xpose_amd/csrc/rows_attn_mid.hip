@@ -5,6 +5,10 @@
 // A wave's keys go through LDS of its own, 32 at a time, K and V in one buffer each: the
 // next K is on its way from the end of the scores on, the next V from the end of the
 // values on, and no barrier is needed until the waves' sums meet.
+//
+// Latency bounds it: a step of a wave's 32 keys takes 2.4 us (its products 0.25), with one wave
+// a SIMD at 256 dims, two at less. A prompt of 2000 rows of 4 heads over 1 of 256 with a
+// window of 512 takes 32 us; as tiles of 128 rows 47, as a list 48.
 #include "xp_rows_attn32.hpp"
 
 namespace xp {

@@ -1,6 +1,17 @@
 // Attention of many rows (prompts and their chunks): a workgroup's four waves take
 // 32 rows each of a tile and share the keys' tiles in LDS.
 // The 32 rows of a wave are xp_rows_attn32.hpp's.
+//
+// 32 rows a wave, as many as two waves a SIMD have registers for at 128 dims, and four waves
+// to a tile of keys: each wave reads the whole tile, 32 KB for 1024 cycles of products, which
+// the LDS gives at about the rate of the products. K and V go to LDS without passing through
+// registers, one tile ahead. Instruction issue bounds it: at 128 dims the products take 0.47 of
+// a SIMD's cycles, what else there is for its two waves (an exponential a score, maximum,
+// sum, packing) 0.46, and they hardly meet. A prompt of 16384, 16 heads over 2 of 128 in bf16,
+// takes 1120 to 1180 us (930 to 980 TFLOP/s; a library's product of 8192 1224), 8192 at 64 dims 650, at
+// 256 dims (one wave a SIMD) 540 to 610; chunks of 512 over 15000 in bf16 880, f16 810, e4m3 670, i8
+// 570 (each wave widens all keys itself). Tried: a wave's priority raised for its products
+// or for its softmax (both 5 % slower), three waves a SIMD at 64 dims (spills; lists 20 % slower).
 #include "xp_rows_attn32.hpp"
 
 namespace xp {

@@ -1,5 +1,5 @@
 // What the kernels of attention over packed rows share (rows_attn_few.hip,
-// rows_attn_tile.hip, rows_attention.hip): their places in the deal, operands of
+// rows_attn_mid.hip, rows_attn_tile.hip, rows_attention.hip): their places in the deal, operands of
 // the matrix instructions, tiles on their way to LDS.
 #pragma once
 
@@ -256,10 +256,11 @@ __device__ __forceinline__ u32x2 widen4(uint32_t w) {
 // place c ^ f(key), so that what a wave reads at once meets each of the 64 banks once: a
 // line of 256 bytes, which holds up to four short rows. Of K a lane reads a chunk, 16
 // following keys at a time (as f has it 6.7 cycles a read, with eight values of f for 16
-// keys 8.3; rows of 32 chunks all the same get eight, as sixteen take more registers
-// than there are: a prompt of 8192, 16 heads over 4 of 256, 892 us so, 988 with sixteen). V is read transposed, half a wave at a time: 16-bit elements as four
-// following keys of 64 bytes in the kernels of 32 rows (HI 3), eight of 32 in that of 16
-// (HI 4); 8-bit ones as keys 0..3 and 8..11 of 32 bytes, and keys 0..7 and 16..23 of 16.
+// keys 8.3; rows of 32 chunks all the same get eight, as sixteen take more registers than
+// there are: a prompt of 8192, 16 heads over 4 of 256, 892 us so, 988 with sixteen). V is
+// read transposed, half a wave at a time: 16-bit elements as four following keys of 64
+// bytes in the kernels of 32 rows (HI 3), eight of 32 in that of 16 (HI 4); 8-bit ones as
+// keys 0..3 and 8..11 of 32 bytes, and keys 0..7 and 16..23 of 16.
 template <int CHUNKS>
 __device__ __forceinline__ constexpr uint32_t swizzle_k(uint32_t key) {
     return CHUNKS >= 32 ? ((key & 3u) << 1) | ((key >> 2) & 1u) : CHUNKS == 16 ? key & 15u : CHUNKS == 8 ? (key >> 1) & 7u : (key >> 2) & 3u;
