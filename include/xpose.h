@@ -476,7 +476,8 @@ int xp_paged_kv_read(const xp_paged_kv* c, const xp_paged_seqs* s, const xp_rows
  * queries are taken as they are, BF16 and F32 ones over a cache of another
  * type as powers of two times F16 terms (F32: two terms). out has q's heads
  * and elem and must not overlap q or the cache. More than
- * 2^24 tiles of 16 to 128 rows are refused.
+ * 2^24 tiles of 16 to 128 rows are refused. Each workgroup walks all
+ * sequences: calls of more than a thousand or so are faster split.
  *
  * workspace: where there are too few rows for the device's CUs, or lengths too
  * different, the keys are split, and the parts meet in workspace_bytes (at

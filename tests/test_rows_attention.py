@@ -496,3 +496,12 @@ def test_workspace_of_one_sequence_suffices_for_any_number(xh, heads, kvh, dim):
         need = xh.attention_workspace(most, 1, heads, kvh, dim)
         for n in (x for x in sizes if x <= most):
             assert all(xh.attention_workspace(n, b, heads, kvh, dim) <= need for b in (1, 2, 5, 64, 4000))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,past", [([1, 1], [700, 30]), ([5, 1], [20, 300])])
+def test_gpu_attention_paged_more_heads_than_a_tile_has_rows(xp, new, past):
+    for positions in (1024, 8192):
+        table, pages = wide_table(new, past, 16, positions)
+        c = Paged(xp, new, past, 200, 1, 64, "f16", "f16", 16, n_pages=pages, table=table)
+        c.check(c.run())

@@ -8,7 +8,7 @@
 // registers, one tile ahead. Instruction issue bounds it: at 128 dims the products take 0.47 of
 // a SIMD's cycles, what else there is for its two waves (an exponential a score, maximum,
 // sum, packing) 0.46, and they hardly meet. A prompt of 16384, 16 heads over 2 of 128 in bf16,
-// takes 1120 to 1180 us (930 to 980 TFLOP/s; a library's product of 8192 1224), 8192 at 64 dims 650, at
+// takes 1100 to 1180 us (930 to 1000 TFLOP/s; a library's product of 8192 1224), 8192 at 64 dims 650, at
 // 256 dims (one wave a SIMD) 540 to 610; chunks of 512 over 15000 in bf16 880, f16 810, e4m3 670, i8
 // 570 (each wave widens all keys itself). Tried: a wave's priority raised for its products
 // or for its softmax (both 5 % slower), three waves a SIMD at 64 dims (spills; lists 20 % slower).
